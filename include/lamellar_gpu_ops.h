@@ -489,6 +489,53 @@ lmr_status_t lmr_scatter_results(const void* d_in, const uint32_t* d_pos, uint64
 lmr_status_t lmr_reduce(lmr_ctx_t* ctx, uint32_t dtype, uint32_t op, const void* d_shard, uint64_t len,
                         uint64_t* d_out, uint8_t* d_has, lmr_stream_t stream);
 
+/* ---------------------------------------------------------------- rows
+ * The batched load / add / store with a whole row as the record: a table of `rows` rows of
+ * row_len elements in HBM, a batch of n row indices and (add, store) n rows of values. This PE's
+ * rows only; a table over several PEs packs its records by owner first (lmr_pack) and calls these
+ * at the owner.
+ *   d_idx       n row indices, signed, 4 or 8 bytes each (index_size). An index equal to `pad`
+ *               (has_pad != 0) names no row: load writes zeros, add and store skip the record.
+ *               Any other index outside [0, rows) does the same and raises LMR_ERRBIT_OOB.
+ *   values      n rows of row_len elements of val_type / out_type (LMR_ROW_F32, _F16 or _BF16),
+ *               `stride` elements apart; add and store also take stride 0: one row for every record.
+ *               They must not overlap the table.
+ * Arithmetic is f32, rounded once (to nearest, ties to even) where a narrower type is written.
+ * Nothing is allocated and nothing waits; every call may be captured into a graph. Calls on one
+ * table from different streams must be ordered by the caller. n <= LMR_ROW_MAX_BATCH. */
+#define LMR_ROW_MAX_LEN (1u << 18)
+#define LMR_ROWS_MAX 0xFFFFFFF0ull
+#define LMR_ROW_MAX_BATCH (1ull << 30)
+typedef struct {
+    void* data;          /* device pointer: row r starts at element r * row_len */
+    float* scales;       /* 8-bit types: rows x (row_len / group) scales; otherwise unused */
+    uint32_t* claims;    /* rows words, zero before the first lmr_rows_store and left zero by each;
+                            NULL: no row occurs twice in one store */
+    uint64_t rows;       /* <= LMR_ROWS_MAX */
+    uint64_t row_len;    /* 1 .. LMR_ROW_MAX_LEN elements */
+    uint32_t type;       /* lmr_row_type_t */
+    uint32_t group;      /* 8-bit types: elements per scale, divides row_len */
+} lmr_rows_t;
+/* out[t, :] = scale * table[idx[t], :] */
+lmr_status_t lmr_rows_load(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,
+                           int has_pad, int64_t pad, float scale, void* d_out, uint32_t out_type, uint64_t out_stride,
+                           lmr_stream_t stream);
+/* table[r, :] += scale * (sum of vals[t, :] over the records t of row r), for every row named: the
+ * records of a row are summed in f32 in an order that the indices alone decide, so equal calls give
+ * equal bits. Tables of 8-bit codes: LMR_E_UNSUPPORTED. d_work: lmr_rows_add_workspace bytes
+ * (16-byte aligned), the call's own until it has run on the stream; LMR_E_WORKSPACE when short. */
+uint64_t lmr_rows_add_workspace(const lmr_rows_t* table, uint64_t n);
+lmr_status_t lmr_rows_add(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,
+                          int has_pad, int64_t pad, float scale, const void* d_vals, uint32_t val_type, uint64_t val_stride,
+                          void* d_work, uint64_t work_bytes, lmr_stream_t stream);
+/* table[idx[t], :] = vals[t, :]; of several records of one row the last one is stored. 8-bit
+ * tables: per group, scale = max(max|x| / Q, 2^-126) with Q = 127 (I8) or 448 (E4M3) and code =
+ * x / scale rounded to the nearest code, each rounding in f32; an infinity or NaN makes the group's
+ * scale NaN. */
+lmr_status_t lmr_rows_store(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,
+                            int has_pad, int64_t pad, const void* d_vals, uint32_t val_type, uint64_t val_stride,
+                            lmr_stream_t stream);
+
 /* ---------------------------------------------------------------- AM wire format
  * The op AMs as the running runtime puts them in a lamellae buffer (SURVEY.md 8(a)
  * a17, 8(f) ranks 1 and 4): bincode legacy (little endian, fixed-width integers,

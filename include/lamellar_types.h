@@ -87,6 +87,15 @@ typedef enum { LMR_DIST_BLOCK = 0, LMR_DIST_CYCLIC = 1 } lmr_distribution_t;
  * "max", "min"; src/array/unsafe.rs:1414-1557). */
 typedef enum { LMR_REDUCE_SUM = 0, LMR_REDUCE_PROD = 1, LMR_REDUCE_MAX = 2, LMR_REDUCE_MIN = 3 } lmr_reduce_op_t;
 
+/* Element types of a table of rows (lmr_rows_*): the floating types a table and the values beside
+ * it may have, then the 8-bit codes a table may hold with one f32 scale per group of elements
+ * (element = code * scale). E4M3 is the OCP 8-bit float (1-4-3, largest 448, no infinities). */
+typedef enum {
+    LMR_ROW_F32 = 0, LMR_ROW_F16 = 1, LMR_ROW_BF16 = 2,
+    LMR_ROW_I8 = 3, LMR_ROW_E4M3 = 4,
+    LMR_NUM_ROW_TYPES = 5
+} lmr_row_type_t;
+
 /* Array kinds that carry the op path (src/array/atomic.rs:28-41, 524-533;
  * impl/src/array_ops.rs:546-572). On the device every kind applies each record
  * atomically per element; the kind only changes the CompareExchangeEps return

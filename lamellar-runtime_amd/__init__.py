@@ -18,10 +18,12 @@ from .world import LamellarWorld, LamellarWorldBuilder, LamellarTeam
 from .array import (AtomicArray, Err, GlobalLockArray, LocalLockArray, Ok, ReadOnlyArray,
                     UnsafeArray)
 from .engine import BatchResult, Owned, run_batch
+from .rows import ROW_TYPES, RowArray
 
 __all__ = [
     "ArrayKind", "ArrayOpCmd", "BatchReturnType", "Distribution", "LmrStatus", "Strategy",
     "DTYPES", "dtype_of", "LamellarError", "DeviceKernels", "LamellarWorld",
     "LamellarWorldBuilder", "LamellarTeam", "AtomicArray", "Err", "GlobalLockArray",
     "LocalLockArray", "Ok", "ReadOnlyArray", "UnsafeArray", "BatchResult", "Owned", "run_batch",
+    "ROW_TYPES", "RowArray",
 ]

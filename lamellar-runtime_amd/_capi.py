@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_int, c_uint8, c_uint32,
+from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_uint8, c_uint32,
                     c_uint64, c_void_p)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -71,6 +71,19 @@ class lmr_transport_t(Structure):
         ("self", c_void_p),
         ("alltoall", ALLTOALL_FN),
         ("alltoallv", ALLTOALLV_FN),
+    ]
+
+
+class lmr_rows_t(Structure):
+    """A table of rows (include/lamellar_gpu_ops.h, "rows")."""
+    _fields_ = [
+        ("data", c_void_p),
+        ("scales", c_void_p),
+        ("claims", c_void_p),
+        ("rows", c_uint64),
+        ("row_len", c_uint64),
+        ("type", c_uint32),
+        ("group", c_uint32),
     ]
 
 
@@ -189,6 +202,13 @@ SIGNATURES = {
     "lmr_apply_msg": (c_int, [c_void_p, c_void_p, c_uint64, AM_RESOLVER_FN, SHARD_RESOLVER_FN, c_void_p, c_void_p,
                               c_uint64, POINTER(c_uint64), POINTER(c_uint64), c_uint32, POINTER(c_uint32),
                               c_void_p]),
+    "lmr_rows_load": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint64, c_int, c_int64, c_float, c_void_p,
+                              c_uint32, c_uint64, c_void_p]),
+    "lmr_rows_add_workspace": (c_uint64, [c_void_p, c_uint64]),
+    "lmr_rows_add": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint64, c_int, c_int64, c_float, c_void_p,
+                             c_uint32, c_uint64, c_void_p, c_uint64, c_void_p]),
+    "lmr_rows_store": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint64, c_int, c_int64, c_void_p, c_uint32,
+                               c_uint64, c_void_p]),
 }
 
 STAGES = ["direct", "mvsi", "bin_count", "scan", "bin_scatter", "tile_apply", "pack",

@@ -1,0 +1,60 @@
+// lmr_rows.hpp — the row operators' arguments and element types (lmr_rows.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <type_traits>
+#include "../../include/lamellar_gpu_ops.h"
+
+namespace lmr {
+
+struct RowTable {
+    void* data;          // rows x row_len elements
+    float* scales;       // 8-bit types: rows x groups
+    uint32_t* claims;    // rows words, zero between calls (null: the caller's rows are distinct)
+    uint64_t rows;
+    uint32_t row_len, type;
+    uint32_t group, groups;   // elements of a group, groups of a row (other types: the whole row, 1)
+};
+struct RowBatch {
+    const void* idx;
+    uint32_t index_size;
+    bool has_pad;
+    int64_t pad;
+    uint64_t n;
+    float scale;
+    uint64_t stride;     // elements between two records' values
+};
+
+struct code_i8 { int8_t b; };
+struct code_e4m3 { uint8_t b; };
+template <typename T> struct is_code { static constexpr bool v = false; };
+template <> struct is_code<code_i8> { static constexpr bool v = true; };
+template <> struct is_code<code_e4m3> { static constexpr bool v = true; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return float(v); }
+__device__ __forceinline__ float to_f32(__bf16 v) { return float(v); }
+__device__ __forceinline__ float to_f32(code_i8 v) { return float(v.b); }
+__device__ __forceinline__ float to_f32(code_e4m3 v) { return __builtin_amdgcn_cvt_f32_fp8(int(v.b), 0); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return T(v); }
+
+// A group's scale from its largest |x| (as bits). The floor keeps 1 / scale finite; an infinity or
+// NaN in the group makes the scale NaN, and the codes 0, so that the whole group reads back as NaN:
+// 8-bit integers have no code for it, and a finite scale would hide it.
+struct GroupScale { float scale, inv; };
+template <typename T>
+__device__ __forceinline__ GroupScale group_scale(uint32_t max_bits) {
+    constexpr float inv_q = is_code<T>::v && std::is_same_v<T, code_i8> ? float(1.0 / 127.0) : float(1.0 / 448.0);
+    if (max_bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
+    const float s = fmaxf(__uint_as_float(max_bits) * inv_q, 1.17549435e-38f);
+    return {s, 1.0f / s};
+}
+template <typename T>
+__device__ __forceinline__ T to_code(float x, const GroupScale& q) {
+    const float y = q.inv == 0.f ? 0.f : x * q.inv;      // |y| <= Q (1 + 2^-22): rounds to a code
+    if constexpr (std::is_same_v<T, code_i8>) return {int8_t(__float2int_rn(y))};
+    else return {uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(y, 0.f, 0, false) & 0xff)};
+}
+
+}  // namespace lmr

@@ -1,0 +1,425 @@
+"""RowArray: a distributed table whose batched ops move whole rows.
+
+The element arrays (array.py) gather, add and store single elements; a table that a model looks up
+by token or a serving process keeps per cached position is used a row at a time. A RowArray has
+`rows` rows of `row_len` elements, its rows distributed over the PEs by the layouts of the element
+arrays (Block or Cyclic), each row whole on its owner's GPU. The element types are f32, f16 and
+bf16, and two 8-bit codes (i8, e4m3) with one f32 scale per `group` elements of a row.
+
+  batch_load_rows(index, scale)        scale * row, as f32 / f16 / bf16: an embedding lookup, or an
+                                       8-bit cache read back
+  batch_add_rows(index, vals, scale)   row += scale * the sum of the batch's values of that row: the
+                                       lookup's gradient (or, with scale = -rate, its update)
+  batch_store_rows(index, vals)        row = vals, quantised when the array holds codes
+
+Sums and scaling are in f32 and round once to the array's (or the result's) type. The outcome of a
+batch depends on its arguments alone: the records of a row are added in an order fixed by the
+indices, and of several records stored to one row the last one of the batch stands, on the highest
+PE that names the row when several do.
+
+Handles are lazy, as the element arrays': spawn() enqueues the batch on torch's current stream,
+value() gives its result for work ordered after it on that stream, block() waits and raises what the
+batch found wrong. With several PEs every batch is collective: all PEs issue the same sequence of
+batches (an empty one where a PE has nothing to send).
+"""
+from __future__ import annotations
+
+import ctypes
+import numbers
+
+import numpy as np
+import torch
+import torch.distributed as dist
+
+from . import _capi
+from .array import _Handle
+from .engine import index_input
+from .kernels import LamellarError, check
+from .types import DTYPES, Distribution, LmrStatus
+
+
+class RowType:
+    """One element type of a row: lmr_row_type_t code, torch dtype, whether it is an 8-bit code."""
+
+    def __init__(self, name, code, torch_dtype, largest=None):
+        self.name, self.code, self.torch, self.largest = name, code, torch_dtype, largest
+        self.is_code = largest is not None
+
+    def __repr__(self):
+        return f"RowType({self.name})"
+
+
+ROW_TYPES = {t.name: t for t in (
+    RowType("f32", 0, torch.float32), RowType("f16", 1, torch.float16), RowType("bf16", 2, torch.bfloat16),
+    RowType("i8", 3, torch.int8, 127.0), RowType("e4m3", 4, torch.float8_e4m3fn, 448.0))}
+_BY_TORCH = {t.torch: t for t in ROW_TYPES.values()}
+MAX_ROW_LEN = 1 << 18                     # LMR_ROW_MAX_LEN
+_INT = (torch.int64, torch.int32)
+
+
+def row_type_of(t) -> RowType:
+    r = t if isinstance(t, RowType) else ROW_TYPES.get(t) if isinstance(t, str) else _BY_TORCH.get(t)
+    if r is None:
+        raise LamellarError(LmrStatus.UNSUPPORTED, f"no row element type {t!r} ({', '.join(ROW_TYPES)})")
+    return r
+
+
+def _value_type(t) -> RowType:
+    r = row_type_of(t)
+    if r.is_code:
+        raise LamellarError(LmrStatus.UNSUPPORTED, f"values are f32, f16 or bf16, not {r.name}")
+    return r
+
+
+class RowsHandle(_Handle):
+    """A batch of rows: spawn() enqueues it, value() its result without waiting, block() the result
+    once the device has finished (raising its errors)."""
+
+    def __init__(self, array, launch):
+        self._array, self._launch = array, launch
+        self._res = None
+        self._launched = False
+
+    def spawn(self):
+        if not self._launched:
+            self._launched = True
+            launch, self._launch = self._launch, None      # its tensors live as long as the stream needs them
+            self._res = launch()
+        return self
+
+    def value(self):
+        return self.spawn()._res
+
+    _value = value
+
+
+class _Table:
+    """lmr_rows_t over tensors that the caller keeps alive."""
+
+    def __init__(self, data, scales, claims, rows, row_len, rtype, group):
+        self.data, self.scales, self.claims = data, scales, claims
+        self.rows, self.row_len, self.rtype, self.group = rows, row_len, rtype, group
+        self.c = _capi.lmr_rows_t(data.data_ptr(), scales.data_ptr() if scales is not None else None,
+                                  claims.data_ptr() if claims is not None else None, rows, row_len, rtype.code,
+                                  group or 0)
+        self.ptr = ctypes.addressof(self.c)
+        self.lo = data.data_ptr()
+        self.hi = self.lo + data.numel() * data.element_size()
+
+    def overlaps(self, t, n):
+        """Whether t (n rows of row_len) reaches into the table's rows."""
+        if n == 0:
+            return False
+        lo = t.data_ptr()
+        return lo < self.hi and self.lo < lo + ((n - 1) * t.stride(0) + self.row_len) * t.element_size()
+
+
+class RowArray:
+    """A table of `rows` x `row_len` elements distributed by rows; zero-filled when made."""
+
+    def __init__(self, team, rows, row_len, distribution=Distribution.Block, dtype="f32", group=None):
+        self._set_up(team, int(rows), int(row_len), distribution, row_type_of(dtype), group)
+        n, dev = self.num_rows_local(), team.kernels.device
+        data = torch.zeros(n, self.row_len, dtype=torch.uint8 if self.rtype.is_code else self.rtype.torch, device=dev)
+        scales = torch.zeros(n, self.row_len // self.group, device=dev) if self.rtype.is_code else None
+        self._adopt(data, scales)
+
+    @classmethod
+    def new(cls, team, rows, row_len, distribution=Distribution.Block, dtype="f32", group=None):
+        """As the element arrays' `new`: a handle whose block() gives the array."""
+        class _New:
+            def block(_self):
+                return cls(team, rows, row_len, distribution, dtype, group)
+        return _New()
+
+    @classmethod
+    def from_tensor(cls, team, data, scales=None, dtype=None, rows=None, distribution=Distribution.Block):
+        """An array over memory that the caller already has: `data`, this PE's rows (2-D, contiguous,
+        on the team's device), shared, not copied. 8-bit codes come as int8, float8_e4m3fn, or uint8
+        with `dtype`, and with `scales` (rows x groups, f32). `rows`: the rows of all PEs (the default:
+        this PE's, at one PE)."""
+        if not isinstance(data, torch.Tensor) or data.dim() != 2 or not data.is_contiguous():
+            raise LamellarError(LmrStatus.INVALID, "from_tensor takes a contiguous 2-D tensor of rows")
+        rt = row_type_of(data.dtype if dtype is None else dtype)
+        if data.dtype != rt.torch and not (rt.is_code and data.dtype == torch.uint8):
+            raise LamellarError(LmrStatus.INVALID, f"{data.dtype} holds no {rt.name}")
+        if _device_of(data) != _device_of(team.kernels):
+            raise LamellarError(LmrStatus.INVALID, f"the rows are on {data.device}, the team on {team.kernels.device}")
+        group = None
+        if rt.is_code:
+            if not isinstance(scales, torch.Tensor) or scales.dim() != 2 or scales.dtype != torch.float32 or \
+                    not scales.is_contiguous() or scales.device != data.device or scales.shape[0] != data.shape[0] or \
+                    scales.shape[1] == 0 or data.shape[1] % scales.shape[1]:
+                raise LamellarError(LmrStatus.INVALID, "8-bit rows need contiguous f32 scales, rows x groups, beside them")
+            group = data.shape[1] // scales.shape[1]
+        elif scales is not None:
+            raise LamellarError(LmrStatus.INVALID, f"{rt.name} rows have no scales")
+        if rows is None:
+            if team.num_pes() > 1:
+                raise LamellarError(LmrStatus.INVALID, "with several PEs from_tensor needs the rows of all of them")
+            rows = data.shape[0]
+        a = object.__new__(cls)
+        a._set_up(team, int(rows), int(data.shape[1]), distribution, rt, group)
+        if a.num_rows_local() != data.shape[0]:
+            raise LamellarError(LmrStatus.LENGTH, f"{data.shape[0]} rows here, {a.num_rows_local()} by the layout")
+        a._adopt(data, scales)
+        return a
+
+    def _set_up(self, team, rows, row_len, distribution, rt, group):
+        if rows < 1 or row_len < 1 or row_len > MAX_ROW_LEN:
+            raise LamellarError(LmrStatus.INVALID, f"a row array of {rows} x {row_len} (row_len: 1 to {MAX_ROW_LEN})")
+        if rt.is_code:
+            group = row_len if group is None else int(group)
+            if group < 1 or row_len % group:
+                raise LamellarError(LmrStatus.INVALID, f"groups of {group} do not divide rows of {row_len}")
+        elif group is not None:
+            raise LamellarError(LmrStatus.INVALID, f"{rt.name} rows have no groups")
+        self.team, self.rtype, self.row_len, self.group = team, rt, row_len, group
+        self.layout = _capi.lmr_layout_t()
+        check(_capi.lib().lmr_layout_new(ctypes.byref(self.layout), rows, team.num_pes(), team.my_pe(),
+                                         int(distribution)), "lmr_layout_new")
+
+    def _adopt(self, data, scales):
+        n = self.num_rows_local()
+        claims = torch.zeros(n, dtype=torch.int32, device=data.device)
+        self._table = _Table(data, scales, claims, n, self.row_len, self.rtype, self.group)
+        self._streams = set()             # streams whose work may still use the tensors when the array is dropped
+        self.team.barrier()
+
+    # ---- layout ----
+    def num_rows(self):
+        return int(self.layout.size)
+
+    def __len__(self):
+        return self.num_rows()
+
+    @property
+    def dtype(self):
+        return self.rtype.name
+
+    def num_pes(self):
+        return self.team.num_pes()
+
+    def my_pe(self):
+        return self.team.my_pe()
+
+    def num_rows_local(self):
+        return int(_capi.lib().lmr_num_elems_pe(ctypes.byref(self.layout), self.team.my_pe()))
+
+    def local_rows(self):
+        """This PE's rows, a tensor over the array's own memory (8-bit rows: their codes)."""
+        return self._table.data.view(self.rtype.torch)
+
+    def local_scales(self):
+        """This PE's scales (rows x groups), a tensor over the array's own memory; None without codes."""
+        return self._table.scales
+
+    def barrier(self):
+        self.team.barrier()
+
+    def wait_all(self):
+        self.team.kernels.synchronize()
+        self.team.kernels.check_errors()
+
+    # ---- batched ops ----
+    def batch_load_rows(self, index, scale=1.0, out_dtype=None, pad=None, out=None):
+        """scale * row for every index, in input order: index.shape + (row_len,). Type: `out_dtype`
+        (the array's own by default; bf16 for 8-bit rows). An index equal to `pad` gives zeros. `out`:
+        a tensor to write instead of a new one; its rows may be strided."""
+        scale, pad = _scale(scale), _pad(pad)
+        if out is not None:
+            rt = _value_type(out.dtype)
+            if out_dtype is not None and _value_type(out_dtype) is not rt:
+                raise LamellarError(LmrStatus.INVALID, f"out is {rt.name}, not {out_dtype}")
+        else:
+            rt = _value_type(out_dtype) if out_dtype is not None else ROW_TYPES["bf16"] if self.rtype.is_code else self.rtype
+        return RowsHandle(self, lambda: self._load(index, scale, rt, pad, out))
+
+    def batch_add_rows(self, index, vals, scale=1.0, pad=None):
+        """row += scale * (sum of the values that name it). vals: index.shape + (row_len,), or one row
+        for every index. 8-bit rows refuse it: a sum of codes has no code."""
+        if self.rtype.is_code:
+            raise LamellarError(LmrStatus.UNSUPPORTED, f"batch_add_rows on {self.rtype.name} rows")
+        scale, pad = _scale(scale), _pad(pad)
+        return RowsHandle(self, lambda: self._write(index, vals, scale, pad, True))
+
+    def batch_store_rows(self, index, vals, pad=None):
+        """row = vals, rounded (f16, bf16) or quantised by groups (i8, e4m3) as it is stored."""
+        pad = _pad(pad)
+        return RowsHandle(self, lambda: self._write(index, vals, 1.0, pad, False))
+
+    # ---- one PE's part, and the exchange ----
+    def _on_stream(self, k):
+        """The current stream will use the array's memory: its reuse waits for that stream."""
+        s = k.stream_id()
+        if s not in self._streams:
+            self._streams.add(s)
+            k.keep_for_stream([t for t in (self._table.data, self._table.scales, self._table.claims) if t is not None])
+
+    def _index(self, k, index):
+        """(1-D index tensor of 4 or 8 bytes, the shape it had)."""
+        if isinstance(index, torch.Tensor):
+            if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+                raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {index.dtype}")
+            shape = index.shape
+            if index.dtype in _INT and index.device == k.device:
+                return index.reshape(-1).contiguous(), shape
+            return index_input(k, index)[1], shape
+        if isinstance(index, numbers.Integral):
+            return torch.tensor([int(index)], dtype=torch.int64, device=k.device), torch.Size([])
+        a = np.asarray(index)
+        if a.size and a.dtype.kind not in "iu":
+            raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {a.dtype}")
+        return index_input(k, a.reshape(-1))[1], torch.Size(a.shape)
+
+    def _values(self, k, vals, n):
+        """(n x row_len tensor whose rows are contiguous, elements between them)."""
+        if not isinstance(vals, torch.Tensor):
+            vals = torch.from_numpy(np.ascontiguousarray(np.asarray(vals), dtype=np.float32))
+        rt = _value_type(vals.dtype)
+        if vals.dim() == 0 or vals.shape[-1] != self.row_len:
+            raise LamellarError(LmrStatus.LENGTH, f"values of {tuple(vals.shape)} for rows of {self.row_len}")
+        if vals.device != k.device:
+            vals = vals.to(k.device)
+        vals = vals.detach().reshape(-1, self.row_len)
+        if vals.shape[0] != n:
+            if vals.shape[0] != 1:
+                raise LamellarError(LmrStatus.LENGTH, f"{n} indices vs {vals.shape[0]} rows of values")
+            vals = vals.expand(n, self.row_len)
+        if (self.row_len > 1 and vals.stride(1) != 1) or (n > 1 and 0 < vals.stride(0) < self.row_len):
+            vals = vals.contiguous()
+        if self._table.overlaps(vals, n):
+            raise LamellarError(LmrStatus.INVALID, "the values lie in the array's own memory")
+        return vals, rt
+
+    def _load(self, index, scale, rt, pad, out):
+        k = self.team.kernels
+        idx, shape = self._index(k, index)
+        n, shape = idx.numel(), shape + (self.row_len,)
+        if out is None:
+            out = torch.empty(shape, dtype=rt.torch, device=k.device)
+            rows = out.view(n, self.row_len) if n else out
+        else:
+            rows = self._out_rows(k, out, shape, n)
+        self._on_stream(k)
+        if self.team.num_pes() > 1:
+            self._exchange_load(k, idx, scale, rt, pad, rows, n)
+        elif n:
+            k.rows_load(self._table, idx, n, pad, scale, rows, rt.code, rows.stride(0))
+        return out
+
+    def _out_rows(self, k, out, shape, n):
+        if out.shape != shape:
+            raise LamellarError(LmrStatus.LENGTH, f"out is {tuple(out.shape)}, the batch {tuple(shape)}")
+        if out.device != k.device:
+            raise LamellarError(LmrStatus.INVALID, f"out is on {out.device}, the team on {k.device}")
+        if n == 0:
+            return out
+        try:
+            rows = out.detach().view(n, self.row_len)
+        except RuntimeError:
+            rows = None
+        if rows is None or (self.row_len > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < self.row_len):
+            raise LamellarError(LmrStatus.INVALID, f"out's rows are not contiguous and evenly spaced: strides {out.stride()}")
+        if self._table.overlaps(rows, n):
+            raise LamellarError(LmrStatus.INVALID, "out lies in the array's own memory")
+        return rows
+
+    def _write(self, index, vals, scale, pad, add):
+        k = self.team.kernels
+        idx, _ = self._index(k, index)
+        n = idx.numel()
+        vals, rt = self._values(k, vals, n)
+        self._on_stream(k)
+        if self.team.num_pes() > 1:
+            idx, vals, pad = self._exchange_values(k, idx, vals, pad)
+            n = idx.numel()
+        if n == 0:
+            return None
+        stride = vals.stride(0) if n > 1 else self.row_len
+        if add:
+            k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride)
+        else:
+            k.rows_store(self._table, idx, n, pad, vals, rt.code, stride)
+        return None
+
+    # Records travel to their rows' owner in input order (the stable pack), sources one after the
+    # other: the owner sees one batch in an order that every run repeats. The counts are read on the
+    # host, so a batch over several PEs waits for its pack.
+    def _pack(self, k, idx, pad):
+        gidx = idx.to(torch.int64)
+        kept = None
+        if pad is not None:
+            kept = (gidx != pad).nonzero().reshape(-1)
+            gidx = gidx[kept]
+        n = int(gidx.numel())
+        loc, _, pos, counts = k.pack(self.layout, gidx, n, None, DTYPES["u8"], 8)
+        sent = [int(c) for c in counts.cpu().tolist()]
+        m = sum(sent)                                   # an index out of bounds is dropped there
+        pos = pos[:m].to(torch.int64)
+        got = _all_to_all(self.team, torch.tensor(sent, dtype=torch.int64, device=k.device).view(-1, 1),
+                          [1] * len(sent), [1] * len(sent))
+        got = [int(c) for c in got.view(-1).cpu().tolist()]
+        loc = loc.view(torch.int64)[:m].view(-1, 1) if m else gidx[:0].view(0, 1)
+        return _all_to_all(self.team, loc, sent, got).view(-1), (pos if kept is None else kept[pos]), sent, got
+
+    def _exchange_load(self, k, idx, scale, rt, pad, rows, n):
+        mine, pos, sent, got = self._pack(k, idx, pad)
+        reply = torch.empty(mine.numel(), self.row_len, dtype=rt.torch, device=k.device)
+        if mine.numel():
+            k.rows_load(self._table, mine, mine.numel(), None, scale, reply, rt.code, self.row_len)
+        reply = _all_to_all(self.team, reply, got, sent)
+        if pos.numel() < n:
+            rows.zero_()                                # pads, and what was out of bounds
+        if not pos.numel():
+            return
+        if rows.stride(0) == self.row_len or n == 1:
+            whole = _Table(rows, None, None, n, self.row_len, rt, None)
+            k.rows_store(whole, pos, pos.numel(), None, reply, rt.code, self.row_len)
+        else:
+            rows[pos] = reply
+
+    def _exchange_values(self, k, idx, vals, pad):
+        mine, pos, sent, got = self._pack(k, idx, pad)
+        return mine, _all_to_all(self.team, vals.index_select(0, pos), sent, got), None
+
+
+def _device_of(x):
+    d = x.device
+    return (d.type, d.index or 0)
+
+
+def _scale(x):
+    if not isinstance(x, (numbers.Real, np.generic)):
+        raise LamellarError(LmrStatus.INVALID, f"scale is a number, not {type(x).__name__}")
+    return float(x)
+
+
+def _pad(x):
+    if x is None:
+        return None
+    if not isinstance(x, numbers.Integral) or not -(1 << 63) <= int(x) < 1 << 63:
+        raise LamellarError(LmrStatus.INVALID, f"pad is an index, not {x!r}")
+    return int(x)
+
+
+def _all_to_all(team, rows, sent, got):
+    """rows (2-D, contiguous): sent[p] of them to PE p, got[p] from PE p, in PE order. On the device
+    over RCCL; a host process group gets host tensors."""
+    width = rows.shape[1]
+    flat = rows.contiguous().view(torch.uint8) if rows.numel() else rows.new_empty(rows.shape[0], width * rows.element_size(), dtype=torch.uint8)
+    if flat.shape[1] % 4 == 0:
+        flat = flat.view(torch.int32) if flat.numel() else flat.new_empty(flat.shape[0], flat.shape[1] // 4, dtype=torch.int32)
+    back = torch.empty(sum(got), flat.shape[1], dtype=flat.dtype, device=flat.device)
+    if flat.is_cuda and dist.get_backend(team.group) != "nccl":
+        host = torch.empty(back.shape, dtype=flat.dtype)
+        dist.all_to_all_single(host, flat.cpu(), output_split_sizes=got, input_split_sizes=sent, group=team.group)
+        back.copy_(host)
+    else:
+        dist.all_to_all_single(back, flat, output_split_sizes=got, input_split_sizes=sent, group=team.group)
+    if back.numel():
+        return back.view(rows.dtype)
+    return back.new_empty(sum(got), width, dtype=rows.dtype)
+
+
+__all__ = ["RowArray", "RowsHandle", "RowType", "ROW_TYPES", "row_type_of"]

@@ -1,0 +1,281 @@
+"""RowArray without a GPU: what it refuses (Python and C entry points), and its exchange over two and
+three PEs (gloo, CPU test double of the device kernels) against the plain forms of rowref.py."""
+import ctypes
+import os
+import sys
+import tempfile
+
+import numpy as np
+import pytest
+import torch
+import torch.multiprocessing as mp
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+from test_dist_gloo import CpuTestKernels  # noqa: E402
+
+
+class CpuRowKernels(CpuTestKernels):
+    """The row operators of one PE in plain torch, records one after the other."""
+
+    def stream_id(self):
+        return 0
+
+    def keep_for_stream(self, tensors):
+        pass
+
+    def pack(self, layout, gidx, n, vals, dt, iw, stable=True, want_pos=True):
+        ok = (gidx >= 0) & (gidx < layout.size)          # out of bounds: reported and dropped
+        if not bool(ok.all()):
+            self.err |= 1
+        kept = ok.nonzero().reshape(-1)
+        loc, v, pos, counts = super().pack(layout, gidx[kept].contiguous(), int(kept.numel()), vals, dt, iw)
+        return loc, v, kept.to(torch.int32)[pos.long()], counts
+
+    def _live(self, table, idx, pad):
+        out = []
+        for t, i in enumerate(idx.tolist()):
+            if i == pad:
+                continue
+            if not 0 <= i < table.rows:
+                self.err |= 1
+                continue
+            out.append((t, i))
+        return out
+
+    def rows_load(self, table, idx, n, pad, scale, out, out_type, stride):
+        import rowref as ref
+        out.zero_()
+        for t, i in self._live(table, idx, pad):
+            v = table.data[i]
+            if table.rtype.is_code:
+                v = ref.codes_f64(v, table.rtype.name).float() * table.scales[i].repeat_interleave(table.group)
+            out[t] = (v.float() * scale).to(out.dtype)
+
+    def rows_add(self, table, idx, n, pad, scale, vals, val_type, stride):
+        for t, i in self._live(table, idx, pad):
+            table.data[i] = (table.data[i].float() + scale * vals[t].float()).to(table.data.dtype)
+
+    def rows_store(self, table, idx, n, pad, vals, val_type, stride):
+        import rowref as ref
+        for t, i in self._live(table, idx, pad):
+            if table.rtype.is_code:
+                table.data[i], table.scales[i] = (x[0] for x in ref.quantise(vals[t:t + 1], table.rtype.name, table.group))
+            else:
+                table.data[i] = vals[t].to(table.data.dtype)
+
+
+@pytest.fixture(scope="module")
+def team(lam):
+    return lam.LamellarWorldBuilder().with_kernels(CpuRowKernels).build().team()
+
+
+def refused(lam, status, f, *a, **k):
+    with pytest.raises(lam.LamellarError) as e:
+        f(*a, **k)
+    assert e.value.status == status, e.value
+
+
+INVALID, OOB, UNSUPPORTED, LENGTH = 1, 2, 5, 8
+
+
+def test_refused_arrays(lam, team):
+    R = lam.RowArray
+    for rows, width in [(0, 4), (4, 0), (-1, 4), (4, (1 << 18) + 1)]:
+        refused(lam, INVALID, R, team, rows, width)
+    refused(lam, UNSUPPORTED, R, team, 4, 4, dtype="f64")
+    refused(lam, UNSUPPORTED, R, team, 4, 4, dtype="u8")
+    refused(lam, INVALID, R, team, 4, 10, dtype="i8", group=4)
+    refused(lam, INVALID, R, team, 4, 10, dtype="e4m3", group=0)
+    refused(lam, INVALID, R, team, 4, 10, dtype="bf16", group=5)
+    F = R.from_tensor
+    refused(lam, INVALID, F, team, torch.zeros(4))
+    refused(lam, INVALID, F, team, torch.zeros(4, 6)[:, :3])
+    refused(lam, INVALID, F, team, np.zeros((4, 6)))
+    refused(lam, UNSUPPORTED, F, team, torch.zeros(4, 6, dtype=torch.float64))
+    refused(lam, UNSUPPORTED, F, team, torch.zeros(4, 6, dtype=torch.uint8))          # codes of which type?
+    refused(lam, INVALID, F, team, torch.zeros(4, 6), dtype="bf16")
+    refused(lam, INVALID, F, team, torch.zeros(4, 6), scales=torch.ones(4, 1))
+    codes = torch.zeros(4, 6, dtype=torch.int8)
+    for s in (None, torch.ones(4), torch.ones(3, 2), torch.ones(4, 4), torch.ones(4, 2, dtype=torch.float64),
+              torch.ones(4, 0), torch.ones(2, 4).t()):
+        refused(lam, INVALID, F, team, codes, scales=s)
+    refused(lam, LENGTH, F, team, torch.zeros(4, 6), rows=5)
+    a = F(team, codes, scales=torch.ones(4, 2))
+    assert (a.dtype, a.group, len(a), a.row_len) == ("i8", 3, 4, 6) and a.local_rows().data_ptr() == codes.data_ptr()
+    assert R.new(team, 3, 5, dtype="e4m3").block().group == 5
+
+
+def test_refused_batches(lam, team):
+    a = lam.RowArray(team, 10, 6)
+    c = lam.RowArray(team, 10, 6, dtype="i8", group=3)
+    v = torch.ones(3, 6)
+    for h in (lambda i, **k: a.batch_load_rows(i, **k).block(), lambda i, **k: a.batch_add_rows(i, v, **k).block(),
+              lambda i, **k: c.batch_store_rows(i, v, **k).block()):
+        refused(lam, INVALID, h, torch.ones(3))
+        refused(lam, INVALID, h, [0.5, 1.0, 2.0])
+        refused(lam, INVALID, h, torch.ones(3, dtype=torch.bool))
+        refused(lam, INVALID, h, [0, 1, 2], pad=0.5)
+        refused(lam, INVALID, h, [0, 1, 2], pad=1 << 63)
+        refused(lam, OOB, h, [0, 10, 2])
+        refused(lam, OOB, h, [0, -1, 2])
+    a.local_rows().zero_()                               # (records within bounds beside those were applied)
+    refused(lam, UNSUPPORTED, c.batch_add_rows, [0, 1, 2], v)
+    refused(lam, INVALID, a.batch_load_rows, [0], scale="2")
+    refused(lam, INVALID, a.batch_add_rows, [0], v, scale=torch.ones(1))
+    refused(lam, UNSUPPORTED, a.batch_load_rows, [0], out_dtype="f64")
+    refused(lam, UNSUPPORTED, a.batch_load_rows, [0], out_dtype="i8")
+    refused(lam, UNSUPPORTED, a.batch_load_rows, [0], out=torch.empty(1, 6, dtype=torch.int32))
+    refused(lam, INVALID, a.batch_load_rows, [0], out=torch.empty(1, 6), out_dtype="bf16")
+    mem = torch.empty(100)
+    for out, status in [(torch.empty(2, 6), LENGTH), (torch.empty(18), LENGTH), (torch.empty(6, 3).t(), INVALID),
+                        (mem.as_strided((3, 6), (4, 1)), INVALID), (mem.as_strided((3, 6), (0, 1)), INVALID),
+                        (a.local_rows()[:3], INVALID)]:
+        refused(lam, status, a.batch_load_rows([0, 1, 2], out=out).spawn)
+    for vals, status in [(torch.ones(2, 6), LENGTH), (torch.ones(3, 5), LENGTH), (torch.tensor(1.0), LENGTH),
+                         (torch.ones(3, 6, dtype=torch.float64), UNSUPPORTED), (torch.ones(3, 6, dtype=torch.int8), UNSUPPORTED),
+                         (torch.ones(3, 6, dtype=torch.int64), UNSUPPORTED), (a.local_rows()[:3], INVALID)]:
+        refused(lam, status, a.batch_add_rows([0, 1, 2], vals).spawn)
+        refused(lam, status, a.batch_store_rows([0, 1, 2], vals).spawn)
+    assert not a.local_rows().any()                      # nothing of the refused was applied
+    with pytest.warns(RuntimeWarning):
+        h = a.batch_load_rows([1])
+        del h
+
+
+def test_one_pe_batches(lam, team):
+    """The calls that are not refused, on the test double."""
+    a = lam.RowArray(team, 10, 4, dtype="bf16")
+    a.batch_store_rows([1, 2, 1], torch.arange(12.0).view(3, 4)).block()
+    assert a.batch_load_rows(1, out_dtype="f32").block().tolist() == [8, 9, 10, 11]
+    a.batch_add_rows([[1], [1]], torch.ones(4), scale=0.5).block()
+    assert a.batch_load_rows([[1, -1]], pad=-1).block().tolist() == [[[9, 10, 11, 12], [0, 0, 0, 0]]]
+    h = a.batch_load_rows([2])
+    assert h.value() is h.spawn().value() is h.block()
+    assert a.batch_add_rows([], torch.ones(0, 4)).block() is None
+
+
+def test_c_entry_refusals(capi, lam):
+    """Argument checks of the C entry points: each call here is turned down before it looks at the
+    context or the device (the context pointer stands for one; nothing reads it)."""
+    from lamellar_runtime_amd._capi import lmr_rows_t
+    ctx = ctypes.c_void_p(64)
+    p = 1 << 20                                          # stands for device memory
+
+    def table(**k):
+        d = dict(data=p, scales=p, claims=p, rows=10, row_len=8, type=0, group=4)
+        d.update(k)
+        return ctypes.byref(lmr_rows_t(**d))
+
+    def load(t, ctx=ctx, idx=p, iw=8, n=3, out=p, ty=0, stride=8):
+        return capi.lmr_rows_load(ctx, t, idx, iw, n, 0, 0, 1.0, out, ty, stride, None)
+
+    def add(t, ctx=ctx, idx=p, iw=8, n=3, out=p, ty=0, stride=8, work=None, nbytes=0):
+        return capi.lmr_rows_add(ctx, t, idx, iw, n, 0, 0, 1.0, out, ty, stride, work, nbytes, None)
+
+    def store(t, ctx=ctx, idx=p, iw=8, n=3, out=p, ty=0, stride=8):
+        return capi.lmr_rows_store(ctx, t, idx, iw, n, 0, 0, out, ty, stride, None)
+
+    for f in (load, add, store):
+        assert f(None) == 1 and f(table(), ctx=None) == 1
+        for bad in (dict(type=5), dict(row_len=0), dict(row_len=(1 << 18) + 1), dict(rows=1 << 32), dict(data=None), dict(data=p + 2),
+                    dict(type=1, data=p + 1), dict(type=3, group=0), dict(type=4, group=3), dict(type=3, scales=None),
+                    dict(type=4, scales=p + 2), dict(claims=p + 2)):
+            assert f(table(**bad)) == 1, (f, bad)
+        for bad in (dict(idx=None), dict(idx=p + 4), dict(iw=2), dict(iw=1), dict(out=None), dict(out=p + 2), dict(ty=1, out=p + 1),
+                    dict(ty=3), dict(stride=7), dict(n=(1 << 30) + 1), dict(stride=(1 << 40) + 1)):
+            assert f(table(), **bad) == 1, (f, bad)
+        if f is not add:
+            assert f(table(), n=0) == 0 and f(table(type=4), n=0, idx=None, out=None) == 0
+    assert load(table(), stride=0) == 1                  # every record's output in one place
+    assert add(table(), n=0) == 0 and add(table(type=3)) == 5 and add(table(type=4), n=0) == 5
+    big = 1 << 16
+    need = capi.lmr_rows_add_workspace(table(), big)
+    if need:
+        assert add(table(), n=big, work=p, nbytes=need - 1) == 7 and add(table(), n=big, work=None, nbytes=need) == 7
+        assert add(table(), n=big, work=p + 4, nbytes=need) == 7
+
+
+# ------------------------------------------------------------------ several PEs
+def _inputs(rank, n, rows, width, seed):
+    g = torch.Generator().manual_seed(seed * 10 + rank)
+    i = torch.randint(rows, (n,), generator=g)
+    return i, torch.randint(-8, 9, (n, width), generator=g).float() / 8
+
+
+def _worker(rank, ws, port, outdir, dist_kind):
+    sys.path.insert(0, ROOT)
+    sys.path.insert(0, os.path.join(ROOT, "tests"))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(ws), LOCAL_RANK=str(rank))
+    from _lamellar_bootstrap import load_package
+    lam = load_package()
+    from test_rows import CpuRowKernels, _inputs
+    world = lam.LamellarWorldBuilder().with_kernels(CpuRowKernels).build()
+    team, res = world.team(), {}
+    rows, width = 23, 6
+    n = [40, 0, 7][rank]                                 # a PE with nothing to send takes part
+    a = lam.RowArray(team, rows, width, dist_kind)
+    i, v = _inputs(rank, n, rows, width, 1)
+    a.batch_add_rows(i, v, scale=0.5).block()
+    team.barrier()
+    res["after_add"] = a.batch_load_rows(torch.arange(rows)).block().numpy()
+    i, _ = _inputs(rank, n, rows, width, 2)
+    i[::3] = -1                                          # places of no row
+    wide = torch.full((n, width + 3), 7.0)
+    out = a.batch_load_rows(i, scale=2.0, pad=-1, out=wide[:, 1:width + 1]).block()
+    res["load_index"], res["loaded"], res["wide"] = i.numpy(), out.numpy(), wide.numpy()
+    team.barrier()
+    i, v = _inputs(rank, n, rows, width, 3)
+    a.batch_store_rows(i, v).block()
+    team.barrier()
+    res["after_store"] = a.batch_load_rows(torch.arange(rows)).block().numpy()
+    c = lam.RowArray(team, 2, width, dist_kind, dtype="e4m3", group=3)     # fewer rows than PEs
+    i, v = _inputs(rank, n, 2, width, 4)
+    c.batch_store_rows(i, v.to(torch.float16)).block()
+    team.barrier()
+    res["codes"] = c.batch_load_rows([[0], [1]], out_dtype="f32").block().numpy()
+    h = a.batch_load_rows([rows if rank == 0 else 1])
+    try:
+        h.block()
+        res["oob"] = np.array(0)
+    except lam.LamellarError as e:
+        res["oob"] = np.array(int(e.status))
+    res["oob_rows"] = h.value().numpy()
+    shard = torch.zeros(a.num_rows_local(), width)
+    b = lam.RowArray.from_tensor(team, shard, rows=rows, distribution=dist_kind)
+    b.batch_add_rows([5], torch.ones(width)).block()
+    team.barrier()
+    res["five"] = b.batch_load_rows([5]).block().numpy()
+    np.savez(os.path.join(outdir, f"pe{rank}.npz"), **res)
+    import torch.distributed as dist
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("ws,dist_kind", [(2, 0), (2, 1), (3, 0), (3, 1)])
+def test_exchange_gloo(ws, dist_kind):
+    import rowref as ref
+    rows, width = 23, 6
+    port = 29900 + ws * 11 + dist_kind * 5 + (os.getpid() % 200)
+    with tempfile.TemporaryDirectory() as d:
+        mp.spawn(_worker, args=(ws, port, d, dist_kind), nprocs=ws, join=True)
+        pe = [{k: torch.from_numpy(v) for k, v in np.load(os.path.join(d, f"pe{r}.npz")).items()} for r in range(ws)]
+    ins = {s: [_inputs(r, [40, 0, 7][r], rows if s < 4 else 2, width, s) for r in range(ws)] for s in (1, 3, 4)}
+    cat = {s: (torch.cat([x[0] for x in ins[s]]), torch.cat([x[1] for x in ins[s]])) for s in ins}
+    exact, _ = ref.add(torch.zeros(rows, width), *cat[1], 0.5)           # eighths: every sum is exact
+    stored = exact.float()
+    for r, t in ref.last_records(cat[3][0], rows).items():
+        stored[r] = cat[3][1][t]
+    codes, scales = ref.quantise(cat[4][1].half(), "e4m3", 3)
+    last = ref.last_records(cat[4][0], 2)
+    for p, r in enumerate(pe):
+        assert torch.equal(r["after_add"].double(), exact)
+        assert torch.equal(r["loaded"].double(), ref.load(exact.float(), r["load_index"], 2.0, pad=-1))
+        assert (r["wide"][:, 0] == 7).all() and (r["wide"][:, width + 1:] == 7).all()
+        assert torch.equal(r["after_store"], stored)
+        for row in (0, 1):
+            exp = ref.load(ref.codes_f64(codes, "e4m3"), torch.tensor([last[row]]), 1.0, scales, 3)
+            assert torch.equal(r["codes"][row, 0].double(), exp[0].float().double())
+        assert int(r["oob"]) == (2 if p == 0 else 0)
+        assert torch.equal(r["oob_rows"][0], torch.zeros(width) if p == 0 else stored[1])
+        assert (r["five"] == ws).all()
