@@ -49,22 +49,347 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
     }
 }
 
-// one block per record: the first record of a row sums the row's records in order
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_some(const T* p, int cnt) {
+    if (cnt >= kChunk) return load_chunk(p);
+    return load_part(p, cnt);
+}
+
+template <typename T>
+__device__ __forceinline__ void add_to_row(T* p, Chunk<T> old, const float (&acc)[kChunk], float scale, int cnt) {
+    float v[kChunk];
+    unpack(old, v);
+#pragma unroll
+    for (int i = 0; i < kChunk; i++) v[i] = fmaf(scale, acc[i], v[i]);
+    if (cnt >= kChunk) store_chunk(p, pack<T>(v));
+    else store_part(p, pack<T>(v), cnt);
+}
+
+// ---------------------------------------------------------------- add, few records
+// One launch: a block per record and 512 columns. Each wave finds the record's row in the whole list
+// (kFewRecords indices, 8 a lane); a record with an earlier one of its row leaves. The first sums the
+// row's records in order, its four waves a quarter each where there are more than four.
+constexpr int kFewRecords = 512;
+
 template <typename T, typename V, int IW>
-__global__ __launch_bounds__(256) void k_rows_add(RowTable tab, RowBatch b, const V* vals, uint32_t* err) {
-    const uint64_t t = blockIdx.x;
-    const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0);
+__global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, const V* vals, uint32_t* err) {
+    __shared__ uint16_t list[kFewRecords];
+    __shared__ float sum[3][64][kChunk + 1];
+    const uint32_t t = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0 && blockIdx.y == 0);
     if (r < 0) return;
-    bool earlier = false;
-    for (uint64_t u = threadIdx.x & 63; u < t; u += 64) earlier |= row_index<IW>(b, u) == r;
-    if (__ballot(earlier)) return;                       // (every wave of the block votes alike)
-    T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
-    for (uint64_t j = threadIdx.x; j < tab.row_len; j += blockDim.x) {
-        float acc = 0.f;
-        for (uint64_t u = t; u < b.n; u++)
-            if (row_index<IW>(b, u) == r) acc += to_f32(vals[u * b.stride + j]);
-        row[j] = from_f32<T>(fmaf(b.scale, acc, to_f32(row[j])));
+    const uint32_t col = (blockIdx.y * 64 + lane) * kChunk;
+    const int cnt = int(tab.row_len) - int(col);
+    T* p = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len + col;
+    Chunk<T> old = load_some(p, w == 0 ? cnt : 0);
+    uint32_t total = 0;
+    bool hit[kFewRecords / 64], earlier = false;
+#pragma unroll
+    for (int i = 0; i < kFewRecords / 64; i++) {
+        const uint32_t u = i * 64 + lane;
+        hit[i] = u < b.n && row_index<IW>(b, u) == r;
+        earlier |= hit[i] && u < t;
     }
+    if (__ballot(earlier)) return;                                 // (alike in every wave)
+#pragma unroll
+    for (int i = 0; i < kFewRecords / 64; i++) {
+        const uint64_t m = __ballot(hit[i]);
+        if (hit[i] && w == 0) list[total + __popcll(m & ((1ull << lane) - 1))] = uint16_t(i * 64 + lane);
+        total += __popcll(m);
+    }
+    __syncthreads();
+    const uint32_t share = total > 4 ? (total + 3) / 4 : total;
+    const uint32_t j0 = min(total, w * share), j1 = min(total, j0 + share);
+    float acc[kChunk] = {};
+    constexpr int U = 4;
+    for (uint32_t j = j0; j < j1; j += U) {
+        Chunk<V> c[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t rec = list[min(j + u, total - 1)];
+            c[u] = load_some(vals + uint64_t(rec) * b.stride + col, j + u < j1 ? cnt : 0);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float v[kChunk];
+            unpack(c[u], v);
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) acc[i] += v[i];
+        }
+    }
+    if (total > 4) {
+        if (w > 0) {
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) sum[w - 1][lane][i] = acc[i];
+        }
+        __syncthreads();
+        if (w == 0) {
+#pragma unroll
+            for (int o = 0; o < 3; o++)
+#pragma unroll
+                for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
+        }
+    }
+    if (w == 0 && cnt > 0) add_to_row(p, old, acc, b.scale, cnt);
+}
+
+// ---------------------------------------------------------------- add, many records
+// The records sorted by row (and by place inside a row), then summed run by run.
+//
+// Sort: least significant digit first, digits of up to 10 bits. A pass is two launches: each block
+// counts the digits of its tile, then places its tile behind what earlier tiles and lower digits
+// take. Records keep their order among equal digits: a wave ranks its 64 records by ballots, waves
+// and tiles follow one another in order.
+constexpr int kSortThreads = 512;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kSortBits = 10;
+constexpr uint32_t kNoRow = 0xffffffffu;
+
+struct SortPass {
+    const uint2* in;      // (row, record); null: the batch's indices
+    uint2* out;
+    uint32_t* hist;       // [tiles][1 << bits], then the digits' totals
+    uint32_t n, shift, bits, tiles;
+    bool summed;          // hist holds prefixes over the tiles (k_rows_prefix)
+};
+
+template <int IW>
+__device__ __forceinline__ uint2 sort_record(const SortPass& p, const RowBatch& b, const RowTable& tab, uint32_t* err, uint32_t j) {
+    if (p.in) return p.in[j];
+    const int64_t r = row_of<IW>(b, j, tab.rows, err, true);
+    return {r < 0 ? uint32_t(tab.rows) : uint32_t(r), j};          // skipped records sort behind every row
+}
+
+template <int IW, int IPT>
+__global__ __launch_bounds__(kSortThreads) void k_rows_count(SortPass p, RowBatch b, RowTable tab, uint32_t* err) {
+    __shared__ uint32_t cnt[1 << kSortBits];
+    const uint32_t nd = 1u << p.bits;
+    for (uint32_t d = threadIdx.x; d < nd; d += kSortThreads) cnt[d] = 0;
+    __syncthreads();
+    const uint32_t j0 = blockIdx.x * (kSortThreads * IPT) + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < IPT; k++) {
+        const uint32_t j = j0 + k * kSortThreads;
+        if (j < p.n) atomicAdd(&cnt[(sort_record<IW>(p, b, tab, err, j).x >> p.shift) & (nd - 1)], 1u);
+    }
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < nd; d += kSortThreads) p.hist[uint64_t(blockIdx.x) * nd + d] = cnt[d];
+}
+
+// many tiles: each digit's counts become the counts of the tiles before, the totals go behind them
+__global__ __launch_bounds__(64) void k_rows_prefix(SortPass p) {
+    const uint32_t nd = 1u << p.bits, d = blockIdx.x * 64 + threadIdx.x;
+    if (d >= nd) return;
+    uint32_t sum = 0, t = 0;
+    for (; t + 16 <= p.tiles; t += 16) {
+        uint32_t c[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) c[i] = p.hist[uint64_t(t + i) * nd + d];
+#pragma unroll
+        for (int i = 0; i < 16; i++) { p.hist[uint64_t(t + i) * nd + d] = sum; sum += c[i]; }
+    }
+    for (; t < p.tiles; t++) {
+        const uint32_t c = p.hist[uint64_t(t) * nd + d];
+        p.hist[uint64_t(t) * nd + d] = sum;
+        sum += c;
+    }
+    p.hist[uint64_t(p.tiles) * nd + d] = sum;
+}
+
+template <int IW, int IPT>
+__global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatch b, RowTable tab, uint32_t* err) {
+    __shared__ uint32_t cnt[kSortWaves][1 << kSortBits];
+    __shared__ uint32_t base[1 << kSortBits];
+    __shared__ uint32_t wsum[kSortWaves];
+    const uint32_t nd = 1u << p.bits, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (uint32_t d = lane; d < nd; d += 64) cnt[w][d] = 0;
+    // what lies before this tile's records of digit d: thread x has digits 2x and 2x + 1
+    uint32_t before[2] = {0, 0}, total[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t d = 2 * threadIdx.x + h;
+        if (d >= nd) continue;
+        if (p.summed) {
+            before[h] = p.hist[uint64_t(blockIdx.x) * nd + d];
+            total[h] = p.hist[uint64_t(p.tiles) * nd + d];
+        } else {
+#pragma unroll 8
+            for (uint32_t t = 0; t < p.tiles; t++) {
+                const uint32_t c = p.hist[uint64_t(t) * nd + d];
+                if (t < blockIdx.x) before[h] += c;
+                total[h] += c;
+            }
+        }
+    }
+    uint32_t run = total[0] + total[1];                            // exclusive scan over the threads
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t o = __shfl_up(run, s, 64);
+        if (int(lane) >= s) run += o;
+    }
+    if (lane == 63) wsum[w] = run;
+    __syncthreads();
+    uint32_t lower = run - total[0] - total[1];
+    for (uint32_t i = 0; i < w; i++) lower += wsum[i];
+    if (2 * threadIdx.x < nd) base[2 * threadIdx.x] = lower + before[0];
+    if (2 * threadIdx.x + 1 < nd) base[2 * threadIdx.x + 1] = lower + total[0] + before[1];
+    // a wave's records are neighbours: IPT rounds of 64
+    const uint32_t j0 = blockIdx.x * (kSortThreads * IPT) + w * (64 * IPT) + lane;
+    uint2 rec[IPT];
+    uint32_t rank[IPT];
+#pragma unroll
+    for (int k = 0; k < IPT; k++)
+        rec[k] = j0 + k * 64 < p.n ? sort_record<IW>(p, b, tab, err, j0 + k * 64) : uint2{kNoRow, 0};
+#pragma unroll
+    for (int k = 0; k < IPT; k++) {
+        const bool live = j0 + k * 64 < p.n;
+        const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
+        uint64_t same = __ballot(live);
+        for (uint32_t i = 0; i < p.bits; i++) {
+            const uint64_t bit = __ballot((d >> i) & 1);
+            same &= (d >> i) & 1 ? bit : ~bit;
+        }
+        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+        const uint32_t had = live ? cnt[w][d] : 0;
+        rank[k] = had + below;
+        __builtin_amdgcn_wave_barrier();                           // every lane has read before one writes
+        if (live && below == 0) cnt[w][d] = had + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < nd; d += kSortThreads) {    // waves in order behind the tile's base
+        uint32_t at = base[d];
+#pragma unroll
+        for (int i = 0; i < kSortWaves; i++) {
+            const uint32_t c = cnt[i][d];
+            cnt[i][d] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < IPT; k++) {
+        const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
+        if (j0 + k * 64 < p.n && to < p.n) p.out[to] = rec[k];     // (indices changed under way: still in bounds)
+    }
+}
+
+// Sum: a group of LPR lanes (8 elements each) takes K neighbours of the sorted records. A row whose
+// records all lie in them is added to the table at once. The parts of a row that reaches past them go
+// to `first` (it began before these K) and `last` (it goes on after them); k_rows_join adds them up.
+struct SumArgs {
+    const uint2* rec;     // sorted (row, record)
+    float* first;         // [tiles][pitch]
+    float* last;
+    uint32_t n, k, tiles, pitch;
+    Divisor chunks;       // column chunks of LPR * 8
+};
+
+template <typename T, typename V, int LPR>
+__global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, const V* vals, SumArgs a) {
+    constexpr int U = 4;
+    uint32_t gid = (blockIdx.x * 256u + threadIdx.x) / LPR;
+    if constexpr (LPR == 64) gid = __builtin_amdgcn_readfirstlane(gid);
+    const uint32_t tile = uint32_t(quotient64(gid, a.chunks));
+    if (tile >= a.tiles) return;
+    const uint32_t col = ((gid - tile * a.chunks.d) * LPR + threadIdx.x % LPR) * kChunk;
+    const int cnt = int(tab.row_len) - int(col);
+    const uint32_t rows = uint32_t(tab.rows), k0 = tile * a.k, k1 = min(a.n, k0 + a.k);
+    bool began = k0 > 0 && a.rec[k0 - 1].x == a.rec[k0].x;         // the run at hand began before this tile
+    float acc[kChunk] = {};
+    bool open = false;                                             // the last record's run goes on
+    for (uint32_t k = k0; k < k1; k += U) {
+        uint2 e[U + 1];
+#pragma unroll
+        for (int u = 0; u <= U; u++) e[u] = k + u < a.n ? a.rec[k + u] : uint2{kNoRow, 0};
+        Chunk<V> c[U];
+        Chunk<T> old[U];
+        bool ends[U], part[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            // (a record past the batch: the caller changed the indices while they were sorted)
+            const bool live = k + u < k1 && e[u].x < rows && e[u].y < a.n;
+            c[u] = load_some(vals + uint64_t(e[u].y) * b.stride + col, live ? cnt : 0);
+            ends[u] = live && e[u].x != e[u + 1].x;
+            part[u] = began;
+            if (ends[u]) began = false;
+            old[u] = load_some(reinterpret_cast<const T*>(tab.data) + uint64_t(e[u].x) * tab.row_len + col,
+                               ends[u] && !part[u] ? cnt : 0);
+            if (live) open = !ends[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float v[kChunk];
+            unpack(c[u], v);
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) acc[i] += v[i];
+            if (!ends[u]) continue;
+            if (cnt > 0) {
+                if (part[u]) {
+                    float* f = a.first + uint64_t(tile) * a.pitch + col;
+#pragma unroll
+                    for (int i = 0; i < kChunk; i++) f[i] = acc[i];
+                } else {
+                    add_to_row(reinterpret_cast<T*>(tab.data) + uint64_t(e[u].x) * tab.row_len + col, old[u], acc, b.scale, cnt);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) acc[i] = 0.f;
+        }
+    }
+    if (open && cnt > 0) {
+        float* f = (began ? a.first : a.last) + uint64_t(tile) * a.pitch + col;
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) f[i] = acc[i];
+    }
+}
+
+// one block per tile and 512 columns: where a run goes on past the tile in which it began, its parts
+// are added in order (four waves take a quarter each) and the row is written
+template <typename T>
+__global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, SumArgs a) {
+    const uint32_t tile = blockIdx.x, rows = uint32_t(tab.rows), k0 = tile * a.k, k1 = k0 + a.k;
+    if (k1 >= a.n) return;
+    const uint32_t row = a.rec[k1 - 1].x;
+    if (row >= rows || a.rec[k1].x != row || (k0 > 0 && a.rec[k0 - 1].x == row)) return;
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    // the last tile that begins inside the run: tiles [lo, ..] begin with `row`, narrowed 64 ways a step
+    uint32_t lo = tile + 1, hi = a.tiles;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+        const uint64_t in = __ballot(at < hi && a.rec[uint64_t(at) * a.k].x == row);
+        const uint32_t good = __popcll(in);                        // (sorted: the true lanes come first)
+        const uint32_t next = lo + good * step;
+        hi = min(hi, next + step);
+        lo = next;
+    }
+    const uint32_t parts = lo - tile + 1, share = parts > 8 ? (parts + 3) / 4 : parts;
+    const uint32_t col = (blockIdx.y * 64 + lane) * kChunk;
+    const int cnt = int(tab.row_len) - int(col);
+    float acc[kChunk] = {};
+    const uint32_t j0 = min(parts, w * share), j1 = min(parts, j0 + share);
+    if (cnt > 0) {
+#pragma unroll 4
+        for (uint32_t j = j0; j < j1; j++) {
+            const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + col;
+            const Chunk<float> c = load_chunk(f);
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) acc[i] += __uint_as_float(c.w[i]);
+        }
+    }
+    __shared__ float sum[3][64][kChunk + 1];
+    if (w > 0) {
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) sum[w - 1][lane][i] = acc[i];
+    }
+    __syncthreads();
+    if (w > 0 || cnt <= 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; o++)
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
+    T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len + col;
+    add_to_row(p, load_some(p, cnt), acc, scale, cnt);
 }
 
 // one block per record; a record that a later one overwrites does nothing
@@ -123,12 +448,91 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
         return hipGetLastError();
     }); }); });
 }
-hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, uint32_t* err, hipStream_t s) {
-    return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
-        hipLaunchKernelGGL((k_rows_add<decltype(t), decltype(v), decltype(iw)::value>), dim3(unsigned(b.n)), dim3(256), 0, s,
-                           tab, b, reinterpret_cast<const decltype(v)*>(vals), err);
+// How a batch of adds runs, and its workspace: two lists of (row, record), the digit counts, and the
+// parts of rows that reach past a group's records.
+struct AddPlan {
+    bool few;
+    uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
+    uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
+    uint32_t pitch;
+    uint64_t rec[2], hist, first, last, bytes;
+};
+AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
+    AddPlan p = {};
+    p.few = n <= kFewRecords;
+    if (p.few) return p;
+    const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
+    p.passes = (key_bits + kSortBits - 1) / kSortBits;
+    p.bits = (key_bits + p.passes - 1) / p.passes;
+    p.ipt = n <= 65536 ? 4 : 16;
+    p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
+    const uint32_t cols = (row_len + kChunk - 1) / kChunk;
+    p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
+    p.chunks = (cols + p.lanes - 1) / p.lanes;
+    // 32 records a group, fewer where that would leave less than about 8 waves per compute unit
+    const uint64_t waves = n * p.chunks * p.lanes / 64;
+    p.k = waves >= 32 * 2048 ? 32 : waves >= 16 * 2048 ? 16 : 8;
+    p.groups = uint32_t((n + p.k - 1) / p.k);
+    p.pitch = cols * kChunk;
+    uint64_t at = 0;
+    auto take = [&at](uint64_t bytes) { const uint64_t o = at; at += (bytes + 255) & ~uint64_t(255); return o; };
+    p.rec[0] = take(n * sizeof(uint2));
+    p.rec[1] = take(p.passes > 1 ? n * sizeof(uint2) : 0);
+    p.hist = take((uint64_t(p.tiles) + 1) << p.bits << 2);
+    p.first = take(uint64_t(p.groups) * p.pitch * 4);
+    p.last = take(uint64_t(p.groups) * p.pitch * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <int IW>
+hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b, uint8_t* work, uint32_t* err, hipStream_t s,
+                        const uint2** sorted) {
+    const uint2* in = nullptr;
+    for (uint32_t i = 0; i < p.passes; i++) {
+        uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
+        SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 64};
+        if (p.ipt == 4) hipLaunchKernelGGL((k_rows_count<IW, 4>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        else hipLaunchKernelGGL((k_rows_count<IW, 16>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
+        if (p.ipt == 4) hipLaunchKernelGGL((k_rows_place<IW, 4>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        else hipLaunchKernelGGL((k_rows_place<IW, 16>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        in = out;
+    }
+    *sorted = in;
+    return hipGetLastError();
+}
+
+hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, void* work, uint32_t* err,
+                      hipStream_t s) {
+    const AddPlan p = add_plan(tab.rows, tab.row_len, b.n);
+    if (p.few)
+        return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
+            hipLaunchKernelGGL((k_rows_add_few<decltype(t), decltype(v), decltype(iw)::value>),
+                               dim3(unsigned(b.n), (tab.row_len + 511) / 512), dim3(256), 0, s, tab, b,
+                               reinterpret_cast<const decltype(v)*>(vals), err);
+            return hipGetLastError();
+        }); }); });
+    uint8_t* w = reinterpret_cast<uint8_t*>(work);
+    const uint2* sorted = nullptr;
+    hipError_t e = by_index(b.index_size, [&](auto iw) { return sort_records<decltype(iw)::value>(p, tab, b, w, err, s, &sorted); });
+    if (e != hipSuccess) return e;
+    const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), uint32_t(b.n), p.k,
+                       p.groups, p.pitch, divisor(p.chunks)};
+    const unsigned blocks = unsigned((uint64_t(p.groups) * p.chunks * p.lanes + 255) / 256);
+    return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) {
+        using T = decltype(t);
+        using V = decltype(v);
+        const V* x = reinterpret_cast<const V*>(vals);
+        switch (p.lanes) {
+        case 8: hipLaunchKernelGGL((k_rows_sum<T, V, 8>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
+        case 16: hipLaunchKernelGGL((k_rows_sum<T, V, 16>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
+        case 32: hipLaunchKernelGGL((k_rows_sum<T, V, 32>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
+        default: hipLaunchKernelGGL((k_rows_sum<T, V, 64>), dim3(blocks), dim3(256), 0, s, tab, b, x, a);
+        }
+        hipLaunchKernelGGL((k_rows_join<T>), dim3(p.groups, (tab.row_len + 511) / 512), dim3(256), 0, s, tab, b.scale, a);
         return hipGetLastError();
-    }); }); });
+    }); });
 }
 hipError_t launch_store(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, uint32_t* err, hipStream_t s) {
     return by_row_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
@@ -166,6 +570,7 @@ lmr_status_t check_batch(const lmr_ctx* ctx, const lmr_rows_t* t, const void* id
     const lmr_status_t st = check_table(t);
     if (st != LMR_OK) return st;
     if ((index_size != 4 && index_size != 8) || val_type > LMR_ROW_BF16 || n > LMR_ROW_MAX_BATCH) return LMR_E_INVALID;
+    if (n * t->row_len > LMR_ROW_MAX_VALUES) return LMR_E_INVALID;
     if (n > 0 && (!idx || !vals || !aligned(idx, index_size) || !aligned(vals, type_bytes(val_type)))) return LMR_E_INVALID;
     if (n > 1 && stride < t->row_len && !(may_repeat && stride == 0)) return LMR_E_INVALID;
     if (stride > (uint64_t(1) << 40)) return LMR_E_INVALID;
@@ -228,8 +633,8 @@ lmr_status_t lmr_rows_load(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* 
 }
 
 uint64_t lmr_rows_add_workspace(const lmr_rows_t* table, uint64_t n) {
-    (void)table; (void)n;
-    return 0;
+    if (check_table(table) != LMR_OK || n > LMR_ROW_MAX_BATCH) return 0;
+    return add_plan(table->rows, uint32_t(table->row_len), n).bytes;
 }
 
 lmr_status_t lmr_rows_add(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,
@@ -244,7 +649,7 @@ lmr_status_t lmr_rows_add(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d
     OnDevice dev(ctx->device);
     if (!dev.ok) return LMR_E_HIP;
     return hip_status(launch_add(table_of(table), batch_of(d_idx, index_size, n, has_pad, pad, scale, val_stride), d_vals,
-                                 val_type, ctx->d_err, reinterpret_cast<hipStream_t>(stream)));
+                                 val_type, d_work, ctx->d_err, reinterpret_cast<hipStream_t>(stream)));
 }
 
 lmr_status_t lmr_rows_store(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,

@@ -39,6 +39,77 @@ __device__ __forceinline__ float to_f32(code_e4m3 v) { return __builtin_amdgcn_c
 
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return T(v); }
 
+// Eight elements of a row at a time, from and to addresses aligned to one element (a row of odd
+// length starts anywhere): the device's vector loads take any address, so no aligned form is needed.
+constexpr int kChunk = 8;
+template <typename T> struct Chunk { uint32_t w[kChunk * sizeof(T) / 4]; };
+
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* p) {
+    Chunk<T> c;
+    __builtin_memcpy(&c, p, sizeof(c));
+    return c;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
+    __builtin_memcpy(p, &c, sizeof(c));
+}
+// the first cnt elements (the end of a row)
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_part(const T* p, int cnt) {
+    T e[kChunk] = {};
+#pragma unroll
+    for (int i = 0; i < kChunk; i++) if (i < cnt) e[i] = p[i];
+    Chunk<T> c;
+    __builtin_memcpy(&c, e, sizeof(c));
+    return c;
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, const Chunk<T>& c, int cnt) {
+    T e[kChunk];
+    __builtin_memcpy(e, &c, sizeof(c));
+#pragma unroll
+    for (int i = 0; i < kChunk; i++) if (i < cnt) p[i] = e[i];
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Chunk<T>& c, float (&v)[kChunk]) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) v[i] = __uint_as_float(i & 1 ? c.w[i / 2] & 0xffff0000u : c.w[i / 2] << 16);
+    } else if constexpr (std::is_same_v<T, code_e4m3>) {
+#pragma unroll
+        for (int i = 0; i < kChunk; i += 2) {
+            const auto f = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(int(c.w[i / 4]), true)
+                                 : __builtin_amdgcn_cvt_pk_f32_fp8(int(c.w[i / 4]), false);
+            v[i] = f[0];
+            v[i + 1] = f[1];
+        }
+    } else {
+        T e[kChunk];
+        __builtin_memcpy(e, &c, sizeof(c));
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) v[i] = to_f32(e[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ Chunk<T> pack(const float (&v)[kChunk]) {
+    T e[kChunk];
+#pragma unroll
+    for (int i = 0; i < kChunk; i++) e[i] = from_f32<T>(v[i]);
+    Chunk<T> c;
+    __builtin_memcpy(&c, e, sizeof(c));
+    return c;
+}
+
+// x / d for x < 2^45 (64 bits) and x < 2^17 (32 bits), d < 2^16: multiplication by 2^64 / d (2^32 / d)
+// rounded up is exact while x * d stays below 2^64 (2^32)
+struct Divisor { uint32_t d, m32; uint64_t m64; };
+inline Divisor divisor(uint32_t d) {
+    return {d, d > 1 ? uint32_t((uint64_t(1) << 32) / d + 1) : 0u, d > 1 ? ~uint64_t(0) / d + 1 : 0u};
+}
+__device__ __forceinline__ uint64_t quotient64(uint64_t x, const Divisor& d) { return d.d > 1 ? __umul64hi(x, d.m64) : x; }
+__device__ __forceinline__ uint32_t quotient32(uint32_t x, const Divisor& d) { return d.d > 1 ? __umulhi(x, d.m32) : x; }
+
 // A group's scale from its largest |x| (as bits). The floor keeps 1 / scale finite; an infinity or
 // NaN in the group makes the scale NaN, and the codes 0, so that the whole group reads back as NaN:
 // 8-bit integers have no code for it, and a finite scale would hide it.

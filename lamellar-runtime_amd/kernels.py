@@ -465,35 +465,35 @@ class DeviceKernels:
     # ---- batches of rows (lmr_rows_*): `table` is rows.py's lmr_rows_t with its tensors. They use
     # neither the context's workspace nor its sessions, so an open deferred session stays open.
     def stream_id(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        """The current stream as an integer (0: the default one)."""
+        return torch._C._cuda_getCurrentRawStream(self.device.index or 0)
 
     def keep_for_stream(self, tensors):
         s = torch.cuda.current_stream(self.device)
         for t in tensors:
             t.record_stream(s)
 
-    def rows_load(self, table, idx, n, pad, scale, out, out_type, stride):
+    def rows_load(self, table, idx, n, pad, scale, out, out_type, stride, stream):
         """lmr_rows_load: out[t] = scale * table[idx[t]] (idx: int32 or int64)."""
         st = self.lib.lmr_rows_load(self.ctx, table.ptr, idx.data_ptr(), idx.element_size(), n, pad is not None, pad or 0,
-                                    scale, out.data_ptr(), out_type, stride, self.stream_id())
+                                    scale, out.data_ptr(), out_type, stride, stream)
         if st:
             check(st, "lmr_rows_load")
 
-    def rows_add(self, table, idx, n, pad, scale, vals, val_type, stride):
+    def rows_add(self, table, idx, n, pad, scale, vals, val_type, stride, stream):
         """lmr_rows_add: table[idx[t]] += scale * vals[t], its workspace from torch's allocator (the
         stream's own, and a captured graph's own)."""
         need = self.lib.lmr_rows_add_workspace(table.ptr, n)
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         st = self.lib.lmr_rows_add(self.ctx, table.ptr, idx.data_ptr(), idx.element_size(), n, pad is not None, pad or 0,
-                                   scale, vals.data_ptr(), val_type, stride, work.data_ptr() if need else None, need,
-                                   self.stream_id())
+                                   scale, vals.data_ptr(), val_type, stride, work.data_ptr() if need else None, need, stream)
         if st:
             check(st, "lmr_rows_add")
 
-    def rows_store(self, table, idx, n, pad, vals, val_type, stride):
+    def rows_store(self, table, idx, n, pad, vals, val_type, stride, stream):
         """lmr_rows_store: table[idx[t]] = vals[t]."""
         st = self.lib.lmr_rows_store(self.ctx, table.ptr, idx.data_ptr(), idx.element_size(), n, pad is not None, pad or 0,
-                                     vals.data_ptr(), val_type, stride, self.stream_id())
+                                     vals.data_ptr(), val_type, stride, stream)
         if st:
             check(st, "lmr_rows_store")
 

@@ -250,20 +250,23 @@ class RowArray:
 
     # ---- one PE's part, and the exchange ----
     def _on_stream(self, k):
-        """The current stream will use the array's memory: its reuse waits for that stream."""
+        """The current stream, which will use the array's memory: its reuse waits for that stream."""
         s = k.stream_id()
         if s not in self._streams:
             self._streams.add(s)
             k.keep_for_stream([t for t in (self._table.data, self._table.scales, self._table.claims) if t is not None])
+        return s
 
     def _index(self, k, index):
         """(1-D index tensor of 4 or 8 bytes, the shape it had)."""
         if isinstance(index, torch.Tensor):
-            if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
-                raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {index.dtype}")
             shape = index.shape
             if index.dtype in _INT and index.device == k.device:
-                return index.reshape(-1).contiguous(), shape
+                if len(shape) != 1 or not index.is_contiguous():
+                    index = index.reshape(-1).contiguous()
+                return index, shape
+            if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+                raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {index.dtype}")
             return index_input(k, index)[1], shape
         if isinstance(index, numbers.Integral):
             return torch.tensor([int(index)], dtype=torch.int64, device=k.device), torch.Size([])
@@ -277,6 +280,11 @@ class RowArray:
         if not isinstance(vals, torch.Tensor):
             vals = torch.from_numpy(np.ascontiguousarray(np.asarray(vals), dtype=np.float32))
         rt = _value_type(vals.dtype)
+        if vals.shape == (n, self.row_len) and vals.device == k.device and vals.stride(1) == 1 and \
+                vals.stride(0) >= self.row_len:
+            if self._table.overlaps(vals, n):
+                raise LamellarError(LmrStatus.INVALID, "the values lie in the array's own memory")
+            return vals, rt
         if vals.dim() == 0 or vals.shape[-1] != self.row_len:
             raise LamellarError(LmrStatus.LENGTH, f"values of {tuple(vals.shape)} for rows of {self.row_len}")
         if vals.device != k.device:
@@ -295,22 +303,27 @@ class RowArray:
     def _load(self, index, scale, rt, pad, out):
         k = self.team.kernels
         idx, shape = self._index(k, index)
-        n, shape = idx.numel(), shape + (self.row_len,)
+        n, shape = idx.numel(), (*shape, self.row_len)
+        alone = self.team.num_pes() == 1
+        stride = self.row_len
         if out is None:
-            out = torch.empty(shape, dtype=rt.torch, device=k.device)
-            rows = out.view(n, self.row_len) if n else out
+            rows = out = torch.empty(shape, dtype=rt.torch, device=k.device)
+            if len(shape) != 2:
+                rows = out.view(n, self.row_len)
         else:
             rows = self._out_rows(k, out, shape, n)
-        self._on_stream(k)
-        if self.team.num_pes() > 1:
+            if n > 1:
+                stride = rows.stride(0)
+        stream = self._on_stream(k)
+        if not alone:
             self._exchange_load(k, idx, scale, rt, pad, rows, n)
         elif n:
-            k.rows_load(self._table, idx, n, pad, scale, rows, rt.code, rows.stride(0))
+            k.rows_load(self._table, idx, n, pad, scale, rows, rt.code, stride, stream)
         return out
 
     def _out_rows(self, k, out, shape, n):
         if out.shape != shape:
-            raise LamellarError(LmrStatus.LENGTH, f"out is {tuple(out.shape)}, the batch {tuple(shape)}")
+            raise LamellarError(LmrStatus.LENGTH, f"out is {tuple(out.shape)}, the batch {shape}")
         if out.device != k.device:
             raise LamellarError(LmrStatus.INVALID, f"out is on {out.device}, the team on {k.device}")
         if n == 0:
@@ -330,7 +343,7 @@ class RowArray:
         idx, _ = self._index(k, index)
         n = idx.numel()
         vals, rt = self._values(k, vals, n)
-        self._on_stream(k)
+        stream = self._on_stream(k)
         if self.team.num_pes() > 1:
             idx, vals, pad = self._exchange_values(k, idx, vals, pad)
             n = idx.numel()
@@ -338,9 +351,9 @@ class RowArray:
             return None
         stride = vals.stride(0) if n > 1 else self.row_len
         if add:
-            k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride)
+            k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride, stream)
         else:
-            k.rows_store(self._table, idx, n, pad, vals, rt.code, stride)
+            k.rows_store(self._table, idx, n, pad, vals, rt.code, stride, stream)
         return None
 
     # Records travel to their rows' owner in input order (the stable pack), sources one after the
@@ -367,7 +380,7 @@ class RowArray:
         mine, pos, sent, got = self._pack(k, idx, pad)
         reply = torch.empty(mine.numel(), self.row_len, dtype=rt.torch, device=k.device)
         if mine.numel():
-            k.rows_load(self._table, mine, mine.numel(), None, scale, reply, rt.code, self.row_len)
+            k.rows_load(self._table, mine, mine.numel(), None, scale, reply, rt.code, self.row_len, k.stream_id())
         reply = _all_to_all(self.team, reply, got, sent)
         if pos.numel() < n:
             rows.zero_()                                # pads, and what was out of bounds
@@ -375,7 +388,7 @@ class RowArray:
             return
         if rows.stride(0) == self.row_len or n == 1:
             whole = _Table(rows, None, None, n, self.row_len, rt, None)
-            k.rows_store(whole, pos, pos.numel(), None, reply, rt.code, self.row_len)
+            k.rows_store(whole, pos, pos.numel(), None, reply, rt.code, self.row_len, k.stream_id())
         else:
             rows[pos] = reply
 
@@ -390,14 +403,16 @@ def _device_of(x):
 
 
 def _scale(x):
+    if type(x) is float:
+        return x
     if not isinstance(x, (numbers.Real, np.generic)):
         raise LamellarError(LmrStatus.INVALID, f"scale is a number, not {type(x).__name__}")
     return float(x)
 
 
 def _pad(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int and -(1 << 63) <= x < 1 << 63:
+        return x
     if not isinstance(x, numbers.Integral) or not -(1 << 63) <= int(x) < 1 << 63:
         raise LamellarError(LmrStatus.INVALID, f"pad is an index, not {x!r}")
     return int(x)
