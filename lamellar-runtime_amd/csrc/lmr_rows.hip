@@ -392,30 +392,126 @@ __global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, Su
     add_to_row(p, load_some(p, cnt), acc, scale, cnt);
 }
 
-// one block per record; a record that a later one overwrites does nothing
-template <typename T, typename V, int IW>
-__global__ __launch_bounds__(64) void k_rows_store(RowTable tab, RowBatch b, const V* vals, uint32_t* err) {
-    const uint64_t t = blockIdx.x;
-    const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0);
-    if (r < 0) return;
-    bool later = false;
-    if (tab.claims)
-        for (uint64_t u = t + 1 + threadIdx.x; u < b.n; u += 64) later |= row_index<IW>(b, u) == r;
-    if (__ballot(later)) return;
+// ---------------------------------------------------------------- store
+// Of several records of one row the last is stored. Few records: each looks for its row in the rest of
+// the list. Many: a first launch raises the row's claim to the record's number + 1; the record that
+// finds its own number there stores, and clears the claim.
+constexpr uint64_t kScanRecords = 1024;
+enum { kDistinct, kScanned, kClaimed };
+
+template <int IW>
+__global__ __launch_bounds__(256) void k_rows_claim(RowTable tab, RowBatch b, uint32_t* err) {
+    const uint64_t t = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (t >= b.n) return;
+    const int64_t r = row_of<IW>(b, t, tab.rows, err, true);
+    if (r >= 0) atomicMax(&tab.claims[r], uint32_t(t) + 1);
+}
+
+// a code word of four elements
+template <typename T>
+__device__ __forceinline__ uint32_t to_codes(const float* x, const GroupScale& q) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = q.inv == 0.f ? 0.f : x[i] * q.inv;  // |y| <= Q (1 + 2^-22): rounds to a code
+    if constexpr (std::is_same_v<T, code_i8>) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (uint32_t(__float2int_rn(y[i])) & 0xffu) << (8 * i);
+        return w;
+    } else {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true));
+    }
+}
+__device__ __forceinline__ uint32_t max_bits(const float (&v)[kChunk]) {
+    uint32_t m = 0;                                                // largest |x| as bits: infinities and NaN on top
+#pragma unroll
+    for (int i = 0; i < kChunk; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+}
+__device__ __forceinline__ uint32_t max_over(uint32_t m, uint32_t lanes) {
+    for (uint32_t d = lanes / 2; d; d /= 2) m = max(m, uint32_t(__shfl_xor(int(m), int(d), 64)));
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ void store_codes(T* p, const float (&v)[kChunk], const GroupScale& q, int cnt) {
+    Chunk<T> c;
+    c.w[0] = to_codes<T>(v, q);
+    c.w[1] = to_codes<T>(v + 4, q);
+    if (cnt >= kChunk) store_chunk(p, c);
+    else store_part(p, c, cnt);
+}
+
+// WPR waves per record (1: four records a block). Groups of up to 512 elements: as many lanes as hold
+// one (a power of two) find its largest |x| by shuffles and keep its values in registers. Longer
+// groups are read twice, the second time from cache.
+template <typename T, typename V, int IW, int WPR>
+__global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, const V* vals, uint32_t* err, int how, uint32_t lpg) {
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, part = WPR == 4 ? w : 0;
+    uint64_t t = WPR == 4 ? blockIdx.x : uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(w);
+    if (t >= b.n) return;
+    const int64_t r = row_of<IW>(b, t, tab.rows, err, lane == 0);
+    bool mine = r >= 0;
+    if (how == kScanned) {
+        bool later = false;
+        for (uint64_t u = t + 1 + lane; u < b.n; u += 64) later |= row_index<IW>(b, u) == r;
+        mine = mine && !__ballot(later);
+    } else if (how == kClaimed) {
+        mine = mine && tab.claims[r] == uint32_t(t) + 1;
+        if constexpr (WPR > 1) __syncthreads();                    // every wave has read the claim
+        if (mine && part == 0 && lane == 0) tab.claims[r] = 0;
+    }
+    if (!mine) return;
     T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
     const V* x = vals + t * b.stride;
     if constexpr (!is_code<T>::v) {
-        for (uint64_t j = threadIdx.x; j < tab.row_len; j += 64) row[j] = from_f32<T>(to_f32(x[j]));
+#pragma unroll 4
+        for (uint32_t col = (part * 64 + lane) * kChunk; col < tab.row_len; col += WPR * 64 * kChunk) {
+            const int cnt = int(tab.row_len - col);
+            float v[kChunk];
+            unpack(load_some(x + col, cnt), v);
+            if (cnt >= kChunk) store_chunk(row + col, pack<T>(v));
+            else store_part(row + col, pack<T>(v), cnt);
+        }
+    } else if (lpg) {
+        const uint32_t per = 64 / lpg, in = (lane & (lpg - 1)) * kChunk;
+        for (uint32_t g0 = part * per; g0 < tab.groups; g0 += WPR * per) {
+            const uint32_t g = g0 + lane / lpg, col = g * tab.group + in;
+            const int cnt = g < tab.groups ? int(tab.group) - int(in) : 0;
+            float v[kChunk];
+            unpack(load_some(x + col, cnt), v);
+            const GroupScale q = group_scale<T>(max_over(max_bits(v), lpg));
+            if (cnt > 0) {
+                store_codes(row + col, v, q, cnt);
+                if (in == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
+            }
+        }
     } else {
-        for (uint64_t g = 0; g < tab.groups; g++) {
-            uint32_t m = 0;                              // largest |x| as bits: infinities and NaN above every number
-            for (uint64_t j = threadIdx.x; j < tab.group; j += 64)
-                m = max(m, __float_as_uint(to_f32(x[g * tab.group + j])) & 0x7fffffffu);
-            for (int d = 32; d; d >>= 1) m = max(m, uint32_t(__shfl_xor(int(m), d, 64)));
+        __shared__ uint32_t top[2][4];
+        for (uint32_t g = 0; g < tab.groups; g++) {
+            const V* xg = x + uint64_t(g) * tab.group;
+            T* rg = row + uint64_t(g) * tab.group;
+            uint32_t m = 0;
+#pragma unroll 4
+            for (uint32_t in = (part * 64 + lane) * kChunk; in < tab.group; in += WPR * 64 * kChunk) {
+                float v[kChunk];
+                unpack(load_some(xg + in, int(tab.group - in)), v);
+                m = max(m, max_bits(v));
+            }
+            m = max_over(m, 64);
+            if constexpr (WPR > 1) {                               // (two sets: a wave may be one group ahead)
+                if (lane == 0) top[g & 1][w] = m;
+                __syncthreads();
+                m = max(max(top[g & 1][0], top[g & 1][1]), max(top[g & 1][2], top[g & 1][3]));
+            }
             const GroupScale q = group_scale<T>(m);
-            for (uint64_t j = threadIdx.x; j < tab.group; j += 64)
-                row[g * tab.group + j] = to_code<T>(to_f32(x[g * tab.group + j]), q);
-            if (threadIdx.x == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
+#pragma unroll 4
+            for (uint32_t in = (part * 64 + lane) * kChunk; in < tab.group; in += WPR * 64 * kChunk) {
+                float v[kChunk];
+                unpack(load_some(xg + in, int(tab.group - in)), v);
+                store_codes(rg + in, v, q, int(tab.group - in));
+            }
+            if (part == 0 && lane == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
     }
 }
@@ -535,9 +631,20 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     }); });
 }
 hipError_t launch_store(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, uint32_t* err, hipStream_t s) {
+    const int how = !tab.claims || b.n == 1 ? kDistinct : b.n <= kScanRecords ? kScanned : kClaimed;
+    uint32_t lpg = 0;                                              // lanes that hold a group, 0: longer groups
+    if (tab.group <= 64 * kChunk)
+        for (lpg = 1; lpg * kChunk < tab.group;) lpg *= 2;
+    // four waves share a record where records alone do not fill the card and a row has work for them
+    const bool wide = b.n < 2048 && tab.row_len > 512;
     return by_row_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
-        hipLaunchKernelGGL((k_rows_store<decltype(t), decltype(v), decltype(iw)::value>), dim3(unsigned(b.n)), dim3(64), 0, s,
-                           tab, b, reinterpret_cast<const decltype(v)*>(vals), err);
+        using T = decltype(t);
+        using V = decltype(v);
+        constexpr int IW = decltype(iw)::value;
+        const V* x = reinterpret_cast<const V*>(vals);
+        if (how == kClaimed) hipLaunchKernelGGL((k_rows_claim<IW>), dim3(unsigned((b.n + 255) / 256)), dim3(256), 0, s, tab, b, err);
+        if (wide) hipLaunchKernelGGL((k_rows_store<T, V, IW, 4>), dim3(unsigned(b.n)), dim3(256), 0, s, tab, b, x, err, how, lpg);
+        else hipLaunchKernelGGL((k_rows_store<T, V, IW, 1>), dim3(unsigned((b.n + 3) / 4)), dim3(256), 0, s, tab, b, x, err, how, lpg);
         return hipGetLastError();
     }); }); });
 }

@@ -121,11 +121,4 @@ __device__ __forceinline__ GroupScale group_scale(uint32_t max_bits) {
     const float s = fmaxf(__uint_as_float(max_bits) * inv_q, 1.17549435e-38f);
     return {s, 1.0f / s};
 }
-template <typename T>
-__device__ __forceinline__ T to_code(float x, const GroupScale& q) {
-    const float y = q.inv == 0.f ? 0.f : x * q.inv;      // |y| <= Q (1 + 2^-22): rounds to a code
-    if constexpr (std::is_same_v<T, code_i8>) return {int8_t(__float2int_rn(y))};
-    else return {uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(y, 0.f, 0, false) & 0xff)};
-}
-
 }  // namespace lmr
