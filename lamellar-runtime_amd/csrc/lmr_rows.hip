@@ -33,26 +33,70 @@ __device__ __forceinline__ int64_t row_of(const RowBatch& b, uint64_t t, uint64_
     return i;
 }
 
-// one block per record
-template <typename T, typename O, int IW>
-__global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* out, uint32_t* err) {
-    const uint64_t t = blockIdx.x;
-    const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0);
-    for (uint64_t j = threadIdx.x; j < tab.row_len; j += blockDim.x) {
-        float v = 0.f;
-        if (r >= 0) {
-            v = to_f32(reinterpret_cast<const T*>(tab.data)[uint64_t(r) * tab.row_len + j]);
-            if constexpr (is_code<T>::v) v *= tab.scales[uint64_t(r) * tab.groups + j / tab.group];
-            v *= b.scale;
-        }
-        out[t * b.stride + j] = from_f32<O>(v);
-    }
-}
-
 template <typename T>
 __device__ __forceinline__ Chunk<T> load_some(const T* p, int cnt) {
     if (cnt >= kChunk) return load_chunk(p);
     return load_part(p, cnt);
+}
+
+// A thread moves U chunks of 8 elements. The batch's chunks are numbered row after row and dealt to
+// blocks in runs of 256 U, so that any row length fills the lanes; the row of a chunk is a division by
+// the row's chunks (one in 64 bits per block, one in 32 per chunk, both multiplications).
+template <typename T, typename O, int IW, int U>
+__global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* out, uint32_t* err, Divisor cpr) {
+    const uint64_t base = uint64_t(blockIdx.x) * (256 * U);
+    const uint64_t row0 = quotient64(base, cpr);
+    const uint32_t rem = uint32_t(base - row0 * cpr.d) + threadIdx.x;
+    uint64_t t[U];
+    uint32_t col[U];
+    int64_t r[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t off = rem + u * 256, q = quotient32(off, cpr);
+        t[u] = row0 + q;
+        col[u] = (off - q * cpr.d) * kChunk;
+        r[u] = t[u] < b.n ? row_of<IW>(b, t[u], tab.rows, err, col[u] == 0) : -1;
+    }
+    Chunk<T> c[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const T* p = reinterpret_cast<const T*>(tab.data) + uint64_t(r[u]) * tab.row_len + col[u];
+        const int cnt = r[u] < 0 ? 0 : int(tab.row_len - col[u]);
+        c[u] = load_some(p, cnt);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (t[u] >= b.n) continue;
+        float v[kChunk];
+        unpack(c[u], v);
+        if constexpr (is_code<T>::v) {
+            const uint32_t g = col[u] / tab.group;
+            const float* sc = tab.scales + uint64_t(r[u]) * tab.groups + g;
+            if (r[u] >= 0) {
+                uint32_t left = (g + 1) * tab.group - col[u];              // elements of this group from here
+                float s = *sc;
+#pragma unroll
+                for (int i = 0; i < kChunk; i++) {
+                    if (left == 0) {
+                        left = tab.group;
+                        if (col[u] + i < tab.row_len) s = *++sc;
+                    }
+                    left--;
+                    v[i] *= s;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) v[i] *= b.scale;
+        if (r[u] < 0) {
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) v[i] = 0.f;                   // (a scale of infinity makes no NaN of it)
+        }
+        O* p = out + t[u] * b.stride + col[u];
+        const int cnt = int(tab.row_len - col[u]);
+        if (cnt >= kChunk) store_chunk(p, pack<O>(v));
+        else store_part(p, pack<O>(v), cnt);
+    }
 }
 
 template <typename T>
@@ -537,10 +581,21 @@ hipError_t by_index(uint32_t size, F&& f) {
     return size == 4 ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 8>{});
 }
 
-hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32_t out_type, uint32_t* err, hipStream_t s) {
+hipError_t launch_load(const RowTable& tab, RowBatch b, void* out, uint32_t out_type, uint32_t* err, hipStream_t s) {
+    const Divisor cpr = divisor((tab.row_len + kChunk - 1) / kChunk);
     return by_row_type(tab.type, [&](auto t) { return by_value_type(out_type, [&](auto o) { return by_index(b.index_size, [&](auto iw) {
-        hipLaunchKernelGGL((k_rows_load<decltype(t), decltype(o), decltype(iw)::value>), dim3(unsigned(b.n)), dim3(256), 0, s,
-                           tab, b, reinterpret_cast<decltype(o)*>(out), err);
+        using T = decltype(t);
+        using O = decltype(o);
+        constexpr int IW = decltype(iw)::value;
+        const uint64_t chunks = b.n * cpr.d;
+        // four chunks a thread keep four reads in flight; a batch that would leave compute units
+        // without a block gives each thread one
+        if (chunks >= 2048ull * 256)
+            hipLaunchKernelGGL((k_rows_load<T, O, IW, 4>), dim3(unsigned((chunks + 1023) / 1024)), dim3(256), 0, s, tab, b,
+                               reinterpret_cast<O*>(out), err, cpr);
+        else
+            hipLaunchKernelGGL((k_rows_load<T, O, IW, 1>), dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, s, tab, b,
+                               reinterpret_cast<O*>(out), err, cpr);
         return hipGetLastError();
     }); }); });
 }
