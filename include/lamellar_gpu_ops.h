@@ -502,11 +502,13 @@ lmr_status_t lmr_reduce(lmr_ctx_t* ctx, uint32_t dtype, uint32_t op, const void*
  *               They must not overlap the table.
  * Arithmetic is f32, rounded once (to nearest, ties to even) where a narrower type is written.
  * Nothing is allocated and nothing waits; every call may be captured into a graph. Calls on one
- * table from different streams must be ordered by the caller. n <= LMR_ROW_MAX_BATCH, n * row_len <= LMR_ROW_MAX_VALUES. */
+ * table from different streams must be ordered by the caller. n <= LMR_ROW_MAX_BATCH, n * row_len <= LMR_ROW_MAX_VALUES,
+ * stride <= LMR_ROW_MAX_STRIDE. */
 #define LMR_ROW_MAX_LEN (1u << 18)
 #define LMR_ROWS_MAX 0xFFFFFFF0ull
 #define LMR_ROW_MAX_BATCH (1ull << 25)
 #define LMR_ROW_MAX_VALUES (1ull << 36)
+#define LMR_ROW_MAX_STRIDE 0xFFFFFFFFull
 typedef struct {
     void* data;          /* device pointer: row r starts at element r * row_len */
     float* scales;       /* 8-bit types: rows x (row_len / group) scales; otherwise unused */

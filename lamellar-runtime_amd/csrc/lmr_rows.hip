@@ -11,6 +11,7 @@
 // Arithmetic is f32; each result is rounded once, to the nearest even, when it is written.
 #include "lmr_internal.hpp"
 #include "lmr_rows.hpp"
+#include <algorithm>
 
 namespace lmr {
 namespace {
@@ -21,16 +22,19 @@ __device__ __forceinline__ int64_t row_index(const RowBatch& b, uint64_t t) {
     else return reinterpret_cast<const int64_t*>(b.idx)[t];
 }
 
+// whether index i names a row; one that is neither a row nor a pad is reported (by `lead` threads)
+__device__ __forceinline__ bool is_row(const RowBatch& b, int64_t i, uint64_t rows, uint32_t* err, bool lead) {
+    if (b.has_pad && i == b.pad) return false;
+    if (uint64_t(i) < rows) return true;
+    if (lead) atomicOr(err, LMR_ERRBIT_OOB);
+    return false;
+}
+
 // the record's row, or -1: a pad, or out of bounds (reported by `lead` threads)
 template <int IW>
 __device__ __forceinline__ int64_t row_of(const RowBatch& b, uint64_t t, uint64_t rows, uint32_t* err, bool lead) {
     const int64_t i = row_index<IW>(b, t);
-    if (b.has_pad && i == b.pad) return -1;
-    if (uint64_t(i) >= rows) {
-        if (lead) atomicOr(err, LMR_ERRBIT_OOB);
-        return -1;
-    }
-    return i;
+    return is_row(b, i, rows, err, lead) ? i : -1;
 }
 
 template <typename T>
@@ -41,60 +45,73 @@ __device__ __forceinline__ Chunk<T> load_some(const T* p, int cnt) {
 
 // A thread moves U chunks of 8 elements. The batch's chunks are numbered row after row and dealt to
 // blocks in runs of 256 U, so that any row length fills the lanes; the row of a chunk is a division by
-// the row's chunks (one in 64 bits per block, one in 32 per chunk, both multiplications).
-template <typename T, typename O, int IW, int U>
-__global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* out, uint32_t* err, Divisor cpr) {
+// the row's chunks (one in 64 bits per block, one in 32 per chunk, both multiplications). The result is
+// written past the caches' reuse order: it is as large as the table's rows or larger, and read once.
+// GA: groups of a multiple of 8 elements, so that a chunk has one scale.
+template <typename T, typename O, int IW, int U, bool GA>
+__global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* out, uint32_t* err, Divisor cpr, Divisor cpg) {
     const uint64_t base = uint64_t(blockIdx.x) * (256 * U);
     const uint64_t row0 = quotient64(base, cpr);
-    const uint32_t rem = uint32_t(base - row0 * cpr.d) + threadIdx.x;
-    uint64_t t[U];
-    uint32_t col[U];
-    int64_t r[U];
+    const uint32_t rem = uint32_t(base - row0 * cpr.d) + threadIdx.x, n = uint32_t(b.n) - uint32_t(row0);
+    using I = std::conditional_t<IW == 4, int32_t, int64_t>;
+    const I* idx = reinterpret_cast<const I*>(b.idx) + row0;
+    out += row0 * b.stride;
+    uint32_t t[U], c[U];                                 // record and chunk of it
+    I r[U];
+    bool live[U];
+    // (each step for all U before the next, and no load under a condition that another load decides:
+    // the loads of a step are in flight together)
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t off = rem + u * 256, q = quotient32(off, cpr);
-        t[u] = row0 + q;
-        col[u] = (off - q * cpr.d) * kChunk;
-        r[u] = t[u] < b.n ? row_of<IW>(b, t[u], tab.rows, err, col[u] == 0) : -1;
-    }
-    Chunk<T> c[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const T* p = reinterpret_cast<const T*>(tab.data) + uint64_t(r[u]) * tab.row_len + col[u];
-        const int cnt = r[u] < 0 ? 0 : int(tab.row_len - col[u]);
-        c[u] = load_some(p, cnt);
+        const uint32_t off = rem + u * 256;
+        t[u] = quotient32(off, cpr);
+        c[u] = off - t[u] * cpr.d;
+        r[u] = idx[min(t[u], n - 1)];
     }
 #pragma unroll
+    for (int u = 0; u < U; u++) live[u] = t[u] < n && is_row(b, r[u], tab.rows, err, c[u] == 0);
+    Chunk<T> x[U];
+    float sc[U];
+#pragma unroll
     for (int u = 0; u < U; u++) {
-        if (t[u] >= b.n) continue;
+        const uint64_t row = uint32_t(r[u]);             // (a table has fewer rows than 2^32)
+        if constexpr (is_code<T>::v && GA)
+            sc[u] = *(live[u] ? tab.scales + row * tab.groups + quotient32(c[u], cpg) : reinterpret_cast<const float*>(b.idx));
+        const uint32_t col = c[u] * kChunk;
+        x[u] = load_some(reinterpret_cast<const T*>(tab.data) + row * tab.row_len + col,
+                         live[u] ? int(tab.row_len - col) : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (t[u] >= n) continue;
+        const uint32_t col = c[u] * kChunk;
         float v[kChunk];
-        unpack(c[u], v);
-        if constexpr (is_code<T>::v) {
-            const uint32_t g = col[u] / tab.group;
-            const float* sc = tab.scales + uint64_t(r[u]) * tab.groups + g;
-            if (r[u] >= 0) {
-                uint32_t left = (g + 1) * tab.group - col[u];              // elements of this group from here
+        unpack(x[u], v);
+        if constexpr (is_code<T>::v && !GA) {
+            if (live[u]) {
+                const uint32_t g = col / tab.group;
+                const float* sc = tab.scales + uint64_t(uint32_t(r[u])) * tab.groups + g;
+                uint32_t left = (g + 1) * tab.group - col;                 // elements of this group from here
                 float s = *sc;
 #pragma unroll
                 for (int i = 0; i < kChunk; i++) {
                     if (left == 0) {
                         left = tab.group;
-                        if (col[u] + i < tab.row_len) s = *++sc;
+                        if (col + i < tab.row_len) s = *++sc;
                     }
                     left--;
                     v[i] *= s;
                 }
             }
         }
+        float m = b.scale;
+        if constexpr (is_code<T>::v && GA) m *= sc[u];
+        if (!live[u]) m = 0.f;                           // (times a chunk of zeros)
 #pragma unroll
-        for (int i = 0; i < kChunk; i++) v[i] *= b.scale;
-        if (r[u] < 0) {
-#pragma unroll
-            for (int i = 0; i < kChunk; i++) v[i] = 0.f;                   // (a scale of infinity makes no NaN of it)
-        }
-        O* p = out + t[u] * b.stride + col[u];
-        const int cnt = int(tab.row_len - col[u]);
-        if (cnt >= kChunk) store_chunk(p, pack<O>(v));
+        for (int i = 0; i < kChunk; i++) v[i] *= m;
+        O* p = out + uint64_t(t[u]) * b.stride + col;
+        const int cnt = int(tab.row_len - col);
+        if (cnt >= kChunk) stream_chunk(p, pack<O>(v));
         else store_part(p, pack<O>(v), cnt);
     }
 }
@@ -195,6 +212,7 @@ struct SortPass {
     uint32_t* hist;       // [tiles][1 << bits], then the digits' totals
     uint32_t n, shift, bits, tiles;
     bool summed;          // hist holds prefixes over the tiles (k_rows_prefix)
+    uint32_t* joins;      // the count to clear for k_rows_sum, in the first launch
 };
 
 template <int IW>
@@ -208,6 +226,7 @@ template <int IW, int IPT>
 __global__ __launch_bounds__(kSortThreads) void k_rows_count(SortPass p, RowBatch b, RowTable tab, uint32_t* err) {
     __shared__ uint32_t cnt[1 << kSortBits];
     const uint32_t nd = 1u << p.bits;
+    if (!p.in && blockIdx.x == 0 && threadIdx.x == 0) *p.joins = 0;
     for (uint32_t d = threadIdx.x; d < nd; d += kSortThreads) cnt[d] = 0;
     __syncthreads();
     const uint32_t j0 = blockIdx.x * (kSortThreads * IPT) + threadIdx.x;
@@ -247,21 +266,19 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     __shared__ uint32_t wsum[kSortWaves];
     const uint32_t nd = 1u << p.bits, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (uint32_t d = lane; d < nd; d += 64) cnt[w][d] = 0;
-    // what lies before this tile's records of digit d: thread x has digits 2x and 2x + 1
+    // what lies before this tile's records of a digit: thread x has digits 2x and 2x + 1
     uint32_t before[2] = {0, 0}, total[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const uint32_t d = 2 * threadIdx.x + h;
-        if (d >= nd) continue;
+    if (2 * threadIdx.x < nd) {
+        const uint2* h = reinterpret_cast<const uint2*>(p.hist) + threadIdx.x;
         if (p.summed) {
-            before[h] = p.hist[uint64_t(blockIdx.x) * nd + d];
-            total[h] = p.hist[uint64_t(p.tiles) * nd + d];
+            const uint2 c = h[uint64_t(blockIdx.x) * (nd / 2)], e = h[uint64_t(p.tiles) * (nd / 2)];
+            before[0] = c.x, before[1] = c.y, total[0] = e.x, total[1] = e.y;
         } else {
-#pragma unroll 8
+#pragma unroll 16
             for (uint32_t t = 0; t < p.tiles; t++) {
-                const uint32_t c = p.hist[uint64_t(t) * nd + d];
-                if (t < blockIdx.x) before[h] += c;
-                total[h] += c;
+                const uint2 c = h[t * (nd / 2)];
+                if (t < blockIdx.x) before[0] += c.x, before[1] += c.y;
+                total[0] += c.x, total[1] += c.y;
             }
         }
     }
@@ -275,8 +292,10 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     __syncthreads();
     uint32_t lower = run - total[0] - total[1];
     for (uint32_t i = 0; i < w; i++) lower += wsum[i];
-    if (2 * threadIdx.x < nd) base[2 * threadIdx.x] = lower + before[0];
-    if (2 * threadIdx.x + 1 < nd) base[2 * threadIdx.x + 1] = lower + total[0] + before[1];
+    if (2 * threadIdx.x < nd) {
+        base[2 * threadIdx.x] = lower + before[0];
+        base[2 * threadIdx.x + 1] = lower + total[0] + before[1];
+    }
     // a wave's records are neighbours: IPT rounds of 64
     const uint32_t j0 = blockIdx.x * (kSortThreads * IPT) + w * (64 * IPT) + lane;
     uint2 rec[IPT];
@@ -325,6 +344,7 @@ struct SumArgs {
     const uint2* rec;     // sorted (row, record)
     float* first;         // [tiles][pitch]
     float* last;
+    uint32_t* joins;      // [0]: rows to join, [1 ..]: the tiles in which they begin, in any order
     uint32_t n, k, tiles, pitch;
     Divisor chunks;       // column chunks of LPR * 8
 };
@@ -381,6 +401,7 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
             for (int i = 0; i < kChunk; i++) acc[i] = 0.f;
         }
     }
+    if (open && !began && col == 0) a.joins[1 + atomicAdd(a.joins, 1u)] = tile;
     if (open && cnt > 0) {
         float* f = (began ? a.first : a.last) + uint64_t(tile) * a.pitch + col;
 #pragma unroll
@@ -388,52 +409,57 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
     }
 }
 
-// one block per tile and 512 columns: where a run goes on past the tile in which it began, its parts
-// are added in order (four waves take a quarter each) and the row is written
+// Rows that reach past the tile in which they begin: a block takes such a row and 512 columns at a time
+// and adds its parts in order (four waves a quarter each where there are many). The list's order is
+// no one's: every row is in it once.
 template <typename T>
-__global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, SumArgs a) {
-    const uint32_t tile = blockIdx.x, rows = uint32_t(tab.rows), k0 = tile * a.k, k1 = k0 + a.k;
-    if (k1 >= a.n) return;
-    const uint32_t row = a.rec[k1 - 1].x;
-    if (row >= rows || a.rec[k1].x != row || (k0 > 0 && a.rec[k0 - 1].x == row)) return;
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    // the last tile that begins inside the run: tiles [lo, ..] begin with `row`, narrowed 64 ways a step
-    uint32_t lo = tile + 1, hi = a.tiles;
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
-        const uint64_t in = __ballot(at < hi && a.rec[uint64_t(at) * a.k].x == row);
-        const uint32_t good = __popcll(in);                        // (sorted: the true lanes come first)
-        const uint32_t next = lo + good * step;
-        hi = min(hi, next + step);
-        lo = next;
-    }
-    const uint32_t parts = lo - tile + 1, share = parts > 8 ? (parts + 3) / 4 : parts;
-    const uint32_t col = (blockIdx.y * 64 + lane) * kChunk;
-    const int cnt = int(tab.row_len) - int(col);
-    float acc[kChunk] = {};
-    const uint32_t j0 = min(parts, w * share), j1 = min(parts, j0 + share);
-    if (cnt > 0) {
-#pragma unroll 4
-        for (uint32_t j = j0; j < j1; j++) {
-            const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + col;
-            const Chunk<float> c = load_chunk(f);
-#pragma unroll
-            for (int i = 0; i < kChunk; i++) acc[i] += __uint_as_float(c.w[i]);
-        }
-    }
+__global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, SumArgs a, Divisor wide) {
     __shared__ float sum[3][64][kChunk + 1];
-    if (w > 0) {
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, items = *a.joins * wide.d;
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t which = uint32_t(quotient64(item, wide)), tile = a.joins[1 + which];
+        const uint32_t row = a.rec[uint64_t(tile + 1) * a.k].x;
+        // the last tile that begins inside the run: tiles [lo, ..] begin with `row`, narrowed 64 ways a step
+        uint32_t lo = tile + 1, hi = a.tiles;
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+            const uint64_t in = __ballot(at < hi && a.rec[uint64_t(at) * a.k].x == row);
+            const uint32_t next = lo + __popcll(in) * step;        // (sorted: the true lanes come first)
+            hi = min(hi, next + step);
+            lo = next;
+        }
+        const uint32_t parts = lo - tile + 1, share = parts > 8 ? (parts + 3) / 4 : parts;
+        const uint32_t col = ((item - which * wide.d) * 64 + lane) * kChunk;
+        const int cnt = int(tab.row_len) - int(col);
+        T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len + col;
+        const Chunk<T> old = load_some(p, w == 0 ? cnt : 0);
+        float acc[kChunk] = {};
+        const uint32_t j0 = min(parts, w * share), j1 = min(parts, j0 + share);
+        if (cnt > 0) {
+#pragma unroll 4
+            for (uint32_t j = j0; j < j1; j++) {
+                const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + col;
+                const Chunk<float> c = load_chunk(f);
 #pragma unroll
-        for (int i = 0; i < kChunk; i++) sum[w - 1][lane][i] = acc[i];
+                for (int i = 0; i < kChunk; i++) acc[i] += __uint_as_float(c.w[i]);
+            }
+        }
+        if (parts > 8) {                                           // (alike in the whole block)
+            if (w > 0) {
+#pragma unroll
+                for (int i = 0; i < kChunk; i++) sum[w - 1][lane][i] = acc[i];
+            }
+            __syncthreads();
+            if (w == 0) {
+#pragma unroll
+                for (int o = 0; o < 3; o++)
+#pragma unroll
+                    for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
+            }
+            __syncthreads();
+        }
+        if (w == 0 && cnt > 0) add_to_row(p, old, acc, scale, cnt);
     }
-    __syncthreads();
-    if (w > 0 || cnt <= 0) return;
-#pragma unroll
-    for (int o = 0; o < 3; o++)
-#pragma unroll
-        for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
-    T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len + col;
-    add_to_row(p, load_some(p, cnt), acc, scale, cnt);
 }
 
 // ---------------------------------------------------------------- store
@@ -581,21 +607,29 @@ hipError_t by_index(uint32_t size, F&& f) {
     return size == 4 ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 8>{});
 }
 
-hipError_t launch_load(const RowTable& tab, RowBatch b, void* out, uint32_t out_type, uint32_t* err, hipStream_t s) {
+hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32_t out_type, uint32_t* err, hipStream_t s) {
     const Divisor cpr = divisor((tab.row_len + kChunk - 1) / kChunk);
+    const bool ga = tab.group % kChunk == 0;             // (other types: the whole row is the group, and unused)
+    const Divisor cpg = divisor(ga ? tab.group / kChunk : 1);
     return by_row_type(tab.type, [&](auto t) { return by_value_type(out_type, [&](auto o) { return by_index(b.index_size, [&](auto iw) {
         using T = decltype(t);
         using O = decltype(o);
         constexpr int IW = decltype(iw)::value;
+        O* p = reinterpret_cast<O*>(out);
         const uint64_t chunks = b.n * cpr.d;
         // four chunks a thread keep four reads in flight; a batch that would leave compute units
         // without a block gives each thread one
-        if (chunks >= 2048ull * 256)
-            hipLaunchKernelGGL((k_rows_load<T, O, IW, 4>), dim3(unsigned((chunks + 1023) / 1024)), dim3(256), 0, s, tab, b,
-                               reinterpret_cast<O*>(out), err, cpr);
-        else
-            hipLaunchKernelGGL((k_rows_load<T, O, IW, 1>), dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, s, tab, b,
-                               reinterpret_cast<O*>(out), err, cpr);
+        const bool four = chunks >= 2048ull * 256;
+        const dim3 grid(unsigned(four ? (chunks + 1023) / 1024 : (chunks + 255) / 256));
+        if constexpr (is_code<T>::v) {
+            if (!ga) {
+                if (four) hipLaunchKernelGGL((k_rows_load<T, O, IW, 4, false>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
+                else hipLaunchKernelGGL((k_rows_load<T, O, IW, 1, false>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
+                return hipGetLastError();
+            }
+        }
+        if (four) hipLaunchKernelGGL((k_rows_load<T, O, IW, 4, true>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
+        else hipLaunchKernelGGL((k_rows_load<T, O, IW, 1, true>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
         return hipGetLastError();
     }); }); });
 }
@@ -606,7 +640,7 @@ struct AddPlan {
     uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
     uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
     uint32_t pitch;
-    uint64_t rec[2], hist, first, last, bytes;
+    uint64_t rec[2], hist, joins, first, last, bytes;
 };
 AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     AddPlan p = {};
@@ -615,7 +649,7 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
     p.passes = (key_bits + kSortBits - 1) / kSortBits;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    p.ipt = n <= 65536 ? 4 : 16;
+    p.ipt = n <= 131072 ? 4 : 16;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
@@ -630,6 +664,7 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     p.rec[0] = take(n * sizeof(uint2));
     p.rec[1] = take(p.passes > 1 ? n * sizeof(uint2) : 0);
     p.hist = take((uint64_t(p.tiles) + 1) << p.bits << 2);
+    p.joins = take((uint64_t(p.groups) + 1) * 4);
     p.first = take(uint64_t(p.groups) * p.pitch * 4);
     p.last = take(uint64_t(p.groups) * p.pitch * 4);
     p.bytes = at;
@@ -642,7 +677,8 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
     const uint2* in = nullptr;
     for (uint32_t i = 0; i < p.passes; i++) {
         uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
-        SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 64};
+        SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 64,
+                      reinterpret_cast<uint32_t*>(work + p.joins)};
         if (p.ipt == 4) hipLaunchKernelGGL((k_rows_count<IW, 4>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
         else hipLaunchKernelGGL((k_rows_count<IW, 16>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
         if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
@@ -668,8 +704,10 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     const uint2* sorted = nullptr;
     hipError_t e = by_index(b.index_size, [&](auto iw) { return sort_records<decltype(iw)::value>(p, tab, b, w, err, s, &sorted); });
     if (e != hipSuccess) return e;
-    const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), uint32_t(b.n), p.k,
-                       p.groups, p.pitch, divisor(p.chunks)};
+    const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), reinterpret_cast<uint32_t*>(w + p.joins),
+                       uint32_t(b.n), p.k, p.groups, p.pitch, divisor(p.chunks)};
+    const Divisor wide = divisor((tab.row_len + 64 * kChunk - 1) / (64 * kChunk));
+    const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 2048));
     const unsigned blocks = unsigned((uint64_t(p.groups) * p.chunks * p.lanes + 255) / 256);
     return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) {
         using T = decltype(t);
@@ -681,7 +719,7 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
         case 32: hipLaunchKernelGGL((k_rows_sum<T, V, 32>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
         default: hipLaunchKernelGGL((k_rows_sum<T, V, 64>), dim3(blocks), dim3(256), 0, s, tab, b, x, a);
         }
-        hipLaunchKernelGGL((k_rows_join<T>), dim3(p.groups, (tab.row_len + 511) / 512), dim3(256), 0, s, tab, b.scale, a);
+        hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(256), 0, s, tab, b.scale, a, wide);
         return hipGetLastError();
     }); });
 }
@@ -735,7 +773,7 @@ lmr_status_t check_batch(const lmr_ctx* ctx, const lmr_rows_t* t, const void* id
     if (n * t->row_len > LMR_ROW_MAX_VALUES) return LMR_E_INVALID;
     if (n > 0 && (!idx || !vals || !aligned(idx, index_size) || !aligned(vals, type_bytes(val_type)))) return LMR_E_INVALID;
     if (n > 1 && stride < t->row_len && !(may_repeat && stride == 0)) return LMR_E_INVALID;
-    if (stride > (uint64_t(1) << 40)) return LMR_E_INVALID;
+    if (stride > LMR_ROW_MAX_STRIDE) return LMR_E_INVALID;
     return LMR_OK;
 }
 

@@ -54,6 +54,15 @@ template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
     __builtin_memcpy(p, &c, sizeof(c));
 }
+// the same for data that the caches need not keep
+template <typename T>
+__device__ __forceinline__ void stream_chunk(T* p, const Chunk<T>& c) {
+    typedef uint32_t x4 __attribute__((ext_vector_type(4), aligned(2)));
+    x4 v[sizeof(c) / 16];
+    __builtin_memcpy(v, &c, sizeof(c));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(c) / 16; i++) __builtin_nontemporal_store(v[i], reinterpret_cast<x4*>(p) + i);
+}
 // the first cnt elements (the end of a row)
 template <typename T>
 __device__ __forceinline__ Chunk<T> load_part(const T* p, int cnt) {
