@@ -37,12 +37,6 @@ __device__ __forceinline__ int64_t row_of(const RowBatch& b, uint64_t t, uint64_
     return is_row(b, i, rows, err, lead) ? i : -1;
 }
 
-template <typename T>
-__device__ __forceinline__ Chunk<T> load_some(const T* p, int cnt) {
-    if (cnt >= kChunk) return load_chunk(p);
-    return load_part(p, cnt);
-}
-
 // A thread moves U chunks of 8 elements. The batch's chunks are numbered row after row and dealt to
 // blocks in runs of 256 U, so that any row length fills the lanes; the row of a chunk is a division by
 // the row's chunks (one in 64 bits per block, one in 32 per chunk, both multiplications). The result is
@@ -56,7 +50,7 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
     using I = std::conditional_t<IW == 4, int32_t, int64_t>;
     const I* idx = reinterpret_cast<const I*>(b.idx) + row0;
     out += row0 * b.stride;
-    uint32_t t[U], c[U];                                 // record and chunk of it
+    uint32_t t[U], c[U], col[U];                         // record, chunk of it, where that begins
     I r[U];
     bool live[U];
     // (each step for all U before the next, and no load under a condition that another load decides:
@@ -66,6 +60,7 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
         const uint32_t off = rem + u * 256;
         t[u] = quotient32(off, cpr);
         c[u] = off - t[u] * cpr.d;
+        col[u] = span_of(c[u], tab.row_len).at;
         r[u] = idx[min(t[u], n - 1)];
     }
 #pragma unroll
@@ -77,27 +72,24 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
         const uint64_t row = uint32_t(r[u]);             // (a table has fewer rows than 2^32)
         if constexpr (is_code<T>::v && GA)
             sc[u] = *(live[u] ? tab.scales + row * tab.groups + quotient32(c[u], cpg) : reinterpret_cast<const float*>(b.idx));
-        const uint32_t col = c[u] * kChunk;
-        x[u] = load_some(reinterpret_cast<const T*>(tab.data) + row * tab.row_len + col,
-                         live[u] ? int(tab.row_len - col) : 0);
+        x[u] = fetch(reinterpret_cast<const T*>(tab.data) + row * tab.row_len, col[u], tab.row_len, live[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (t[u] >= n) continue;
-        const uint32_t col = c[u] * kChunk;
         float v[kChunk];
         unpack(x[u], v);
         if constexpr (is_code<T>::v && !GA) {
             if (live[u]) {
-                const uint32_t g = col / tab.group;
+                const uint32_t g = col[u] / tab.group;
                 const float* sc = tab.scales + uint64_t(uint32_t(r[u])) * tab.groups + g;
-                uint32_t left = (g + 1) * tab.group - col;                 // elements of this group from here
+                uint32_t left = (g + 1) * tab.group - col[u];                 // elements of this group from here
                 float s = *sc;
 #pragma unroll
                 for (int i = 0; i < kChunk; i++) {
                     if (left == 0) {
                         left = tab.group;
-                        if (col + i < tab.row_len) s = *++sc;
+                        if (col[u] + i < tab.row_len) s = *++sc;
                     }
                     left--;
                     v[i] *= s;
@@ -109,21 +101,20 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
         if (!live[u]) m = 0.f;                           // (times a chunk of zeros)
 #pragma unroll
         for (int i = 0; i < kChunk; i++) v[i] *= m;
-        O* p = out + uint64_t(t[u]) * b.stride + col;
-        const int cnt = int(tab.row_len - col);
-        if (cnt >= kChunk) stream_chunk(p, pack<O>(v));
-        else store_part(p, pack<O>(v), cnt);
+        O* p = out + uint64_t(t[u]) * b.stride;
+        if (tab.row_len >= kChunk) stream_chunk(p + col[u], pack<O>(v));
+        else put(p, 0, tab.row_len, pack<O>(v));
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void add_to_row(T* p, Chunk<T> old, const float (&acc)[kChunk], float scale, int cnt) {
+template <bool WHOLE = false, typename T>
+__device__ __forceinline__ void add_to_row(T* row, const Span& sp, Chunk<T> old, const float (&acc)[kChunk], float scale) {
     float v[kChunk];
     unpack(old, v);
 #pragma unroll
     for (int i = 0; i < kChunk; i++) v[i] = fmaf(scale, acc[i], v[i]);
-    if (cnt >= kChunk) store_chunk(p, pack<T>(v));
-    else store_part(p, pack<T>(v), cnt);
+    if constexpr (WHOLE) store_chunk(row + sp.at, pack<T>(v));
+    else put_own(row, sp, pack<T>(v));
 }
 
 // ---------------------------------------------------------------- add, few records
@@ -139,10 +130,10 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
     const uint32_t t = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0 && blockIdx.y == 0);
     if (r < 0) return;
-    const uint32_t col = (blockIdx.y * 64 + lane) * kChunk;
-    const int cnt = int(tab.row_len) - int(col);
-    T* p = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len + col;
-    Chunk<T> old = load_some(p, w == 0 ? cnt : 0);
+    const Span sp = span_of(blockIdx.y * 64 + lane, tab.row_len);
+    const bool on = sp.lo < sp.hi;
+    T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
+    const Chunk<T> old = fetch(row, sp.at, tab.row_len, on && w == 0);
     uint32_t total = 0;
     bool hit[kFewRecords / 64], earlier = false;
 #pragma unroll
@@ -168,7 +159,7 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t rec = list[min(j + u, total - 1)];
-            c[u] = load_some(vals + uint64_t(rec) * b.stride + col, j + u < j1 ? cnt : 0);
+            c[u] = fetch(vals + uint64_t(rec) * b.stride, sp.at, tab.row_len, on && j + u < j1);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -191,7 +182,7 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
                 for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
         }
     }
-    if (w == 0 && cnt > 0) add_to_row(p, old, acc, b.scale, cnt);
+    if (w == 0 && on) add_to_row(row, sp, old, acc, b.scale);
 }
 
 // ---------------------------------------------------------------- add, many records
@@ -349,15 +340,20 @@ struct SumArgs {
     Divisor chunks;       // column chunks of LPR * 8
 };
 
-template <typename T, typename V, int LPR>
+// (WHOLE: rows of a multiple of 8 elements, whose chunks do not overlap)
+template <typename T, typename V, int LPR, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, const V* vals, SumArgs a) {
-    constexpr int U = 4;
+    constexpr int U = WHOLE ? 8 : 4;                               // records whose values are in flight together
+    constexpr bool kLong = WHOLE || LPR > 8;                       // (shorter rows take the fewest lanes)
     uint32_t gid = (blockIdx.x * 256u + threadIdx.x) / LPR;
     if constexpr (LPR == 64) gid = __builtin_amdgcn_readfirstlane(gid);
     const uint32_t tile = uint32_t(quotient64(gid, a.chunks));
     if (tile >= a.tiles) return;
-    const uint32_t col = ((gid - tile * a.chunks.d) * LPR + threadIdx.x % LPR) * kChunk;
-    const int cnt = int(tab.row_len) - int(col);
+    const uint32_t chunk = (gid - tile * a.chunks.d) * LPR + threadIdx.x % LPR;
+    const Span sp = WHOLE ? Span{chunk * kChunk, 0, kChunk} : span_of(chunk, tab.row_len);
+    const bool on = WHOLE ? sp.at < tab.row_len : sp.lo < sp.hi;
+    float* const first = a.first + uint64_t(tile) * a.pitch + chunk * kChunk;
+    float* const last = a.last + uint64_t(tile) * a.pitch + chunk * kChunk;
     const uint32_t rows = uint32_t(tab.rows), k0 = tile * a.k, k1 = min(a.n, k0 + a.k);
     bool began = k0 > 0 && a.rec[k0 - 1].x == a.rec[k0].x;         // the run at hand began before this tile
     float acc[kChunk] = {};
@@ -373,12 +369,12 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
         for (int u = 0; u < U; u++) {
             // (a record past the batch: the caller changed the indices while they were sorted)
             const bool live = k + u < k1 && e[u].x < rows && e[u].y < a.n;
-            c[u] = load_some(vals + uint64_t(e[u].y) * b.stride + col, live ? cnt : 0);
+            c[u] = fetch<kLong>(vals + uint64_t(e[u].y) * b.stride, sp.at, tab.row_len, on && live);
             ends[u] = live && e[u].x != e[u + 1].x;
             part[u] = began;
             if (ends[u]) began = false;
-            old[u] = load_some(reinterpret_cast<const T*>(tab.data) + uint64_t(e[u].x) * tab.row_len + col,
-                               ends[u] && !part[u] ? cnt : 0);
+            old[u] = fetch<kLong>(reinterpret_cast<const T*>(tab.data) + uint64_t(e[u].x) * tab.row_len, sp.at, tab.row_len,
+                                  on && ends[u] && !part[u]);
             if (live) open = !ends[u];
         }
 #pragma unroll
@@ -388,25 +384,16 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
 #pragma unroll
             for (int i = 0; i < kChunk; i++) acc[i] += v[i];
             if (!ends[u]) continue;
-            if (cnt > 0) {
-                if (part[u]) {
-                    float* f = a.first + uint64_t(tile) * a.pitch + col;
-#pragma unroll
-                    for (int i = 0; i < kChunk; i++) f[i] = acc[i];
-                } else {
-                    add_to_row(reinterpret_cast<T*>(tab.data) + uint64_t(e[u].x) * tab.row_len + col, old[u], acc, b.scale, cnt);
-                }
+            if (on) {
+                if (part[u]) store_chunk(first, pack<float>(acc));
+                else add_to_row<WHOLE>(reinterpret_cast<T*>(tab.data) + uint64_t(e[u].x) * tab.row_len, sp, old[u], acc, b.scale);
             }
 #pragma unroll
             for (int i = 0; i < kChunk; i++) acc[i] = 0.f;
         }
     }
-    if (open && !began && col == 0) a.joins[1 + atomicAdd(a.joins, 1u)] = tile;
-    if (open && cnt > 0) {
-        float* f = (began ? a.first : a.last) + uint64_t(tile) * a.pitch + col;
-#pragma unroll
-        for (int i = 0; i < kChunk; i++) f[i] = acc[i];
-    }
+    if (open && !began && chunk == 0) a.joins[1 + atomicAdd(a.joins, 1u)] = tile;
+    if (open && on) store_chunk(began ? first : last, pack<float>(acc));
 }
 
 // Rows that reach past the tile in which they begin: a block takes such a row and 512 columns at a time
@@ -429,16 +416,17 @@ __global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, Su
             lo = next;
         }
         const uint32_t parts = lo - tile + 1, share = parts > 8 ? (parts + 3) / 4 : parts;
-        const uint32_t col = ((item - which * wide.d) * 64 + lane) * kChunk;
-        const int cnt = int(tab.row_len) - int(col);
-        T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len + col;
-        const Chunk<T> old = load_some(p, w == 0 ? cnt : 0);
+        const uint32_t chunk = (item - which * wide.d) * 64 + lane;
+        const Span sp = span_of(chunk, tab.row_len);
+        const bool on = sp.lo < sp.hi;
+        T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len;
+        const Chunk<T> old = fetch(p, sp.at, tab.row_len, on && w == 0);
         float acc[kChunk] = {};
         const uint32_t j0 = min(parts, w * share), j1 = min(parts, j0 + share);
-        if (cnt > 0) {
+        if (on) {
 #pragma unroll 4
             for (uint32_t j = j0; j < j1; j++) {
-                const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + col;
+                const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + chunk * kChunk;
                 const Chunk<float> c = load_chunk(f);
 #pragma unroll
                 for (int i = 0; i < kChunk; i++) acc[i] += __uint_as_float(c.w[i]);
@@ -458,7 +446,7 @@ __global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, Su
             }
             __syncthreads();
         }
-        if (w == 0 && cnt > 0) add_to_row(p, old, acc, scale, cnt);
+        if (w == 0 && on) add_to_row(p, sp, old, acc, scale);
     }
 }
 
@@ -504,12 +492,8 @@ __device__ __forceinline__ uint32_t max_over(uint32_t m, uint32_t lanes) {
     return m;
 }
 template <typename T>
-__device__ __forceinline__ void store_codes(T* p, const float (&v)[kChunk], const GroupScale& q, int cnt) {
-    Chunk<T> c;
-    c.w[0] = to_codes<T>(v, q);
-    c.w[1] = to_codes<T>(v + 4, q);
-    if (cnt >= kChunk) store_chunk(p, c);
-    else store_part(p, c, cnt);
+__device__ __forceinline__ Chunk<T> pack_codes(const float (&v)[kChunk], const GroupScale& q) {
+    return {{to_codes<T>(v, q), to_codes<T>(v + 4, q)}};
 }
 
 // WPR waves per record (1: four records a block). Groups of up to 512 elements: as many lanes as hold
@@ -536,25 +520,23 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
     const V* x = vals + t * b.stride;
     if constexpr (!is_code<T>::v) {
 #pragma unroll 4
-        for (uint32_t col = (part * 64 + lane) * kChunk; col < tab.row_len; col += WPR * 64 * kChunk) {
-            const int cnt = int(tab.row_len - col);
+        for (uint32_t c = part * 64 + lane; c * kChunk < tab.row_len; c += WPR * 64) {
+            const uint32_t at = span_of(c, tab.row_len).at;
             float v[kChunk];
-            unpack(load_some(x + col, cnt), v);
-            if (cnt >= kChunk) store_chunk(row + col, pack<T>(v));
-            else store_part(row + col, pack<T>(v), cnt);
+            unpack(fetch(x, at, tab.row_len, true), v);
+            put(row, at, tab.row_len, pack<T>(v));
         }
     } else if (lpg) {
-        const uint32_t per = 64 / lpg, in = (lane & (lpg - 1)) * kChunk;
+        const uint32_t per = 64 / lpg, in = lane & (lpg - 1), at = span_of(in, tab.group).at;
         for (uint32_t g0 = part * per; g0 < tab.groups; g0 += WPR * per) {
-            const uint32_t g = g0 + lane / lpg, col = g * tab.group + in;
-            const int cnt = g < tab.groups ? int(tab.group) - int(in) : 0;
+            const uint32_t g = g0 + lane / lpg;
+            const bool on = g < tab.groups && in * kChunk < tab.group;
             float v[kChunk];
-            unpack(load_some(x + col, cnt), v);
+            unpack(fetch(x + g * tab.group, at, tab.group, on), v);
             const GroupScale q = group_scale<T>(max_over(max_bits(v), lpg));
-            if (cnt > 0) {
-                store_codes(row + col, v, q, cnt);
-                if (in == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
-            }
+            if (!on) continue;
+            put(row + g * tab.group, at, tab.group, pack_codes<T>(v, q));
+            if (in == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
     } else {
         __shared__ uint32_t top[2][4];
@@ -563,9 +545,9 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
             T* rg = row + uint64_t(g) * tab.group;
             uint32_t m = 0;
 #pragma unroll 4
-            for (uint32_t in = (part * 64 + lane) * kChunk; in < tab.group; in += WPR * 64 * kChunk) {
+            for (uint32_t c = part * 64 + lane; c * kChunk < tab.group; c += WPR * 64) {
                 float v[kChunk];
-                unpack(load_some(xg + in, int(tab.group - in)), v);
+                unpack(fetch(xg, span_of(c, tab.group).at, tab.group, true), v);
                 m = max(m, max_bits(v));
             }
             m = max_over(m, 64);
@@ -576,10 +558,11 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
             }
             const GroupScale q = group_scale<T>(m);
 #pragma unroll 4
-            for (uint32_t in = (part * 64 + lane) * kChunk; in < tab.group; in += WPR * 64 * kChunk) {
+            for (uint32_t c = part * 64 + lane; c * kChunk < tab.group; c += WPR * 64) {
+                const uint32_t at = span_of(c, tab.group).at;
                 float v[kChunk];
-                unpack(load_some(xg + in, int(tab.group - in)), v);
-                store_codes(rg + in, v, q, int(tab.group - in));
+                unpack(fetch(xg, at, tab.group, true), v);
+                put(rg, at, tab.group, pack_codes<T>(v, q));
             }
             if (part == 0 && lane == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
@@ -713,12 +696,20 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
         using T = decltype(t);
         using V = decltype(v);
         const V* x = reinterpret_cast<const V*>(vals);
-        switch (p.lanes) {
-        case 8: hipLaunchKernelGGL((k_rows_sum<T, V, 8>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
-        case 16: hipLaunchKernelGGL((k_rows_sum<T, V, 16>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
-        case 32: hipLaunchKernelGGL((k_rows_sum<T, V, 32>), dim3(blocks), dim3(256), 0, s, tab, b, x, a); break;
-        default: hipLaunchKernelGGL((k_rows_sum<T, V, 64>), dim3(blocks), dim3(256), 0, s, tab, b, x, a);
-        }
+        auto sum = [&](auto lanes, auto whole) {
+            hipLaunchKernelGGL((k_rows_sum<T, V, decltype(lanes)::value, decltype(whole)::value>), dim3(blocks), dim3(256), 0, s,
+                               tab, b, x, a);
+        };
+        auto by_lanes = [&](auto whole) {
+            switch (p.lanes) {
+            case 8: sum(std::integral_constant<int, 8>{}, whole); break;
+            case 16: sum(std::integral_constant<int, 16>{}, whole); break;
+            case 32: sum(std::integral_constant<int, 32>{}, whole); break;
+            default: sum(std::integral_constant<int, 64>{}, whole);
+            }
+        };
+        if (tab.row_len % kChunk == 0) by_lanes(std::true_type{});
+        else by_lanes(std::false_type{});
         hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(256), 0, s, tab, b.scale, a, wide);
         return hipGetLastError();
     }); });

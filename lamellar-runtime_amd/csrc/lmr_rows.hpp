@@ -63,22 +63,48 @@ __device__ __forceinline__ void stream_chunk(T* p, const Chunk<T>& c) {
 #pragma unroll
     for (unsigned i = 0; i < sizeof(c) / 16; i++) __builtin_nontemporal_store(v[i], reinterpret_cast<x4*>(p) + i);
 }
-// the first cnt elements (the end of a row)
-template <typename T>
-__device__ __forceinline__ Chunk<T> load_part(const T* p, int cnt) {
-    T e[kChunk] = {};
+// The last chunk of a row whose length is no multiple of 8 is the row's last 8 elements: it overlaps
+// the one before, and [lo, hi) are the elements it has for itself. So every access is one whole vector.
+// A chunk behind the row's end has none. Rows shorter than 8 are one chunk, read element by element.
+struct Span { uint32_t at; int lo, hi; };
+__device__ __forceinline__ Span span_of(uint32_t chunk, uint32_t len) {
+    const uint32_t col = chunk * kChunk;
+    if (len < kChunk) return {0, 0, chunk == 0 ? int(len) : 0};
+    if (col + kChunk <= len) return {col, 0, kChunk};
+    return {len - kChunk, col < len ? kChunk - int(len - col) : kChunk, kChunk};
+}
+// (zeros where `on` is false; LONG: the caller knows that rows have at least 8 elements)
+template <bool LONG = false, typename T>
+__device__ __forceinline__ Chunk<T> fetch(const T* p, uint32_t at, uint32_t len, bool on) {
+    Chunk<T> c = {};
+    if (LONG || len >= kChunk) {
+        if (on) c = load_chunk(p + at);
+    } else if (on) {
+        T e[kChunk] = {};
 #pragma unroll
-    for (int i = 0; i < kChunk; i++) if (i < cnt) e[i] = p[i];
-    Chunk<T> c;
-    __builtin_memcpy(&c, e, sizeof(c));
+        for (int i = 0; i < kChunk; i++) if (i < int(len)) e[i] = p[i];
+        __builtin_memcpy(&c, e, sizeof(c));
+    }
     return c;
 }
 template <typename T>
-__device__ __forceinline__ void store_part(T* p, const Chunk<T>& c, int cnt) {
+__device__ __forceinline__ void put_some(T* p, const Chunk<T>& c, int lo, int hi) {
     T e[kChunk];
     __builtin_memcpy(e, &c, sizeof(c));
 #pragma unroll
-    for (int i = 0; i < kChunk; i++) if (i < cnt) p[i] = e[i];
+    for (int i = 0; i < kChunk; i++) if (i >= lo && i < hi) p[i] = e[i];
+}
+// the whole chunk, where two that overlap write the same values
+template <typename T>
+__device__ __forceinline__ void put(T* p, uint32_t at, uint32_t len, const Chunk<T>& c) {
+    if (len >= kChunk) store_chunk(p + at, c);
+    else put_some(p, c, 0, int(len));
+}
+// its own elements only
+template <typename T>
+__device__ __forceinline__ void put_own(T* p, const Span& s, const Chunk<T>& c) {
+    if (s.lo == 0 && s.hi == kChunk) store_chunk(p + s.at, c);
+    else put_some(p + s.at, c, s.lo, s.hi);
 }
 template <typename T>
 __device__ __forceinline__ void unpack(const Chunk<T>& c, float (&v)[kChunk]) {
