@@ -328,16 +328,17 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     }
 }
 
-// Sum: a group of LPR lanes (8 elements each) takes K neighbours of the sorted records. A row whose
-// records all lie in them is added to the table at once. The parts of a row that reaches past them go
-// to `first` (it began before these K) and `last` (it goes on after them); k_rows_join adds them up.
+// Sum: a group of LPR lanes (8 elements each) takes a tile of K neighbours of the sorted records. A row
+// whose records begin in the tile and end there or in the next one is summed by this group alone and
+// added to the table at once. Only longer runs are cut: their parts go to `last` (the tile in which
+// they begin) and `first` (every later one), and k_rows_join adds them up.
 struct SumArgs {
     const uint2* rec;     // sorted (row, record)
     float* first;         // [tiles][pitch]
     float* last;
     uint32_t* joins;      // [0]: rows to join, [1 ..]: the tiles in which they begin, in any order
-    uint32_t n, k, tiles, pitch;
-    Divisor chunks;       // column chunks of LPR * 8
+    uint32_t n, k, tiles, pitch, lanes;
+    Divisor chunks;       // column chunks of `lanes` * 8
 };
 
 // (WHOLE: rows of a multiple of 8 elements, whose chunks do not overlap)
@@ -355,20 +356,52 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
     float* const first = a.first + uint64_t(tile) * a.pitch + chunk * kChunk;
     float* const last = a.last + uint64_t(tile) * a.pitch + chunk * kChunk;
     const uint32_t rows = uint32_t(tab.rows), k0 = tile * a.k, k1 = min(a.n, k0 + a.k);
-    bool began = k0 > 0 && a.rec[k0 - 1].x == a.rec[k0].x;         // the run at hand began before this tile
+    // record k0 + j, j <= 2K <= 64: where the group is a wave, its lanes hold the tile's records and the
+    // next one's, read at once
+    uint2 held = {kNoRow, 0};
+    uint32_t behind = kNoRow;
+    if constexpr (LPR == 64) {
+        if (k0 + (threadIdx.x & 63) < a.n) held = a.rec[k0 + (threadIdx.x & 63)];
+        if (k0 + 64 < a.n) behind = a.rec[k0 + 64].x;
+    }
+    auto row_at = [&](uint32_t j) -> uint32_t {
+        if constexpr (LPR == 64) return j < 64 ? uint32_t(__builtin_amdgcn_readlane(int(held.x), int(j))) : behind;
+        else return k0 + j < a.n ? a.rec[k0 + j].x : kNoRow;
+    };
+    auto record_at = [&](uint32_t j) -> uint32_t {
+        if constexpr (LPR == 64) return uint32_t(__builtin_amdgcn_readlane(int(held.y), int(j)));
+        else return k0 + j < a.n ? a.rec[k0 + j].y : 0;
+    };
+    const uint32_t before = k0 > 0 ? a.rec[k0 - 1].x : kNoRow, long_before = k0 > a.k ? a.rec[k0 - a.k - 1].x : kNoRow;
+    const uint32_t lead = row_at(0), last_row = row_at(k1 - k0 - 1), next = row_at(k1 - k0), next2 = row_at(2 * a.k);
+    bool began = before == lead;                                   // the run at hand began before this tile
+    uint32_t skip = kNoRow, tail = kNoRow, jend = k1 - k0;
+    // the first run is the tile before's, which goes on into this one to its end
+    if (began && next != lead && long_before != lead) {
+        skip = lead;
+        began = false;
+    }
+    // the last run begins here and ends in the next tile: followed to its end
+    if (last_row == next && before != next && next2 != next) {
+        tail = next;
+        jend = min(a.n, k1 + a.k) - k0;
+    }
     float acc[kChunk] = {};
     bool open = false;                                             // the last record's run goes on
-    for (uint32_t k = k0; k < k1; k += U) {
+    for (uint32_t j = 0; j < jend; j += U) {                       // (K is a multiple of U)
         uint2 e[U + 1];
 #pragma unroll
-        for (int u = 0; u <= U; u++) e[u] = k + u < a.n ? a.rec[k + u] : uint2{kNoRow, 0};
+        for (int u = 0; u < U; u++) e[u] = {row_at(j + u), record_at(j + u)};
+        e[U].x = row_at(j + U);
+        if (j >= a.k && e[0].x != tail) break;
         Chunk<V> c[U];
         Chunk<T> old[U];
         bool ends[U], part[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             // (a record past the batch: the caller changed the indices while they were sorted)
-            const bool live = k + u < k1 && e[u].x < rows && e[u].y < a.n;
+            const bool mine = j < a.k ? e[u].x != skip : e[u].x == tail;
+            const bool live = mine && e[u].x < rows && e[u].y < a.n;
             c[u] = fetch<kLong>(vals + uint64_t(e[u].y) * b.stride, sp.at, tab.row_len, on && live);
             ends[u] = live && e[u].x != e[u + 1].x;
             part[u] = began;
@@ -396,57 +429,80 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
     if (open && on) store_chunk(began ? first : last, pack<float>(acc));
 }
 
-// Rows that reach past the tile in which they begin: a block takes such a row and 512 columns at a time
-// and adds its parts in order (four waves a quarter each where there are many). The list's order is
+// Rows that reach past the tile in which they begin: a wave takes such a row and 512 columns and adds
+// its parts in order. Where there are many parts the block does it together (one row may have every
+// record): each wave, or each group of lanes that hold a short row, takes a share. The list's order is
 // no one's: every row is in it once.
+constexpr uint32_t kWaveParts = 32;
+constexpr uint32_t kJoinWaves = 16;
+
+__device__ __forceinline__ void add_parts(const SumArgs& a, uint32_t tile, uint32_t j0, uint32_t j1, uint32_t chunk, float (&acc)[kChunk]) {
+#pragma unroll 8
+    for (uint32_t j = j0; j < j1; j++) {
+        const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + chunk * kChunk;
+        float v[kChunk];
+        unpack(load_chunk(f), v);
+#pragma unroll
+        for (int i = 0; i < kChunk; i++) acc[i] += v[i];
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_rows_join(RowTable tab, float scale, SumArgs a, Divisor wide) {
-    __shared__ float sum[3][64][kChunk + 1];
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, items = *a.joins * wide.d;
-    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t which = uint32_t(quotient64(item, wide)), tile = a.joins[1 + which];
-        const uint32_t row = a.rec[uint64_t(tile + 1) * a.k].x;
-        // the last tile that begins inside the run: tiles [lo, ..] begin with `row`, narrowed 64 ways a step
-        uint32_t lo = tile + 1, hi = a.tiles;
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
-            const uint64_t in = __ballot(at < hi && a.rec[uint64_t(at) * a.k].x == row);
-            const uint32_t next = lo + __popcll(in) * step;        // (sorted: the true lanes come first)
-            hi = min(hi, next + step);
-            lo = next;
-        }
-        const uint32_t parts = lo - tile + 1, share = parts > 8 ? (parts + 3) / 4 : parts;
-        const uint32_t chunk = (item - which * wide.d) * 64 + lane;
-        const Span sp = span_of(chunk, tab.row_len);
-        const bool on = sp.lo < sp.hi;
-        T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len;
-        const Chunk<T> old = fetch(p, sp.at, tab.row_len, on && w == 0);
-        float acc[kChunk] = {};
-        const uint32_t j0 = min(parts, w * share), j1 = min(parts, j0 + share);
-        if (on) {
-#pragma unroll 4
-            for (uint32_t j = j0; j < j1; j++) {
-                const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + chunk * kChunk;
-                const Chunk<float> c = load_chunk(f);
-#pragma unroll
-                for (int i = 0; i < kChunk; i++) acc[i] += __uint_as_float(c.w[i]);
+__global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, float scale, SumArgs a, Divisor wide) {
+    __shared__ float sum[kJoinWaves][64][kChunk + 1];
+    __shared__ uint32_t many[kJoinWaves];
+    const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), items = *a.joins * wide.d, gap = gridDim.x;
+    for (uint32_t base = blockIdx.x; base < items; base += gap * kJoinWaves) {
+        const uint32_t item = base + gap * w;                      // neighbours go to different blocks
+        uint32_t parts = 0;
+        if (item < items) {
+            const uint32_t which = uint32_t(quotient64(item, wide)), tile = a.joins[1 + which];
+            const uint32_t row = a.rec[uint64_t(tile + 1) * a.k].x;
+            // the last tile that begins inside the run: tiles [lo, ..] begin with `row`, narrowed 64 ways a step
+            uint32_t lo = tile + 1, hi = a.tiles;
+            while (hi - lo > 1) {
+                const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+                const uint64_t in = __ballot(at < hi && a.rec[uint64_t(at) * a.k].x == row);
+                const uint32_t next = lo + __popcll(in) * step;    // (sorted: the true lanes come first)
+                hi = min(hi, next + step);
+                lo = next;
+            }
+            parts = lo - tile + 1;
+            const uint32_t chunk = (item - which * wide.d) * 64 + lane;
+            const Span sp = span_of(chunk, tab.row_len);
+            if (parts <= kWaveParts && sp.lo < sp.hi) {
+                T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len;
+                const Chunk<T> old = fetch(p, sp.at, tab.row_len, true);
+                float acc[kChunk] = {};
+                add_parts(a, tile, 0, parts, chunk, acc);
+                add_to_row(p, sp, old, acc, scale);
             }
         }
-        if (parts > 8) {                                           // (alike in the whole block)
-            if (w > 0) {
+        if (lane == 0) many[w] = parts > kWaveParts ? parts : 0;
+        __syncthreads();
+        for (uint32_t i = 0; i < kJoinWaves; i++) {
+            const uint32_t n = many[i];                            // (alike in the whole block)
+            if (n == 0) continue;
+            const uint32_t which = uint32_t(quotient64(base + gap * i, wide)), tile = a.joins[1 + which];
+            const uint32_t per = 64 / a.lanes, mine = w * per + lane / a.lanes, share = (n + kJoinWaves * per - 1) / (kJoinWaves * per);
+            const uint32_t chunk = (base + gap * i - which * wide.d) * 64 + lane % a.lanes;
+            const Span sp = span_of(chunk, tab.row_len);
+            const bool on = sp.lo < sp.hi;
+            float acc[kChunk] = {};
+            if (on) add_parts(a, tile, min(n, mine * share), min(n, (mine + 1) * share), chunk, acc);
 #pragma unroll
-                for (int i = 0; i < kChunk; i++) sum[w - 1][lane][i] = acc[i];
+            for (int k = 0; k < kChunk; k++) sum[w][lane][k] = acc[k];
+            __syncthreads();
+            if (w == 0 && lane < a.lanes && on) {
+                for (uint32_t o = 1; o < kJoinWaves * per; o++)
+#pragma unroll
+                    for (int k = 0; k < kChunk; k++) acc[k] += sum[o / per][o % per * a.lanes + lane][k];
+                T* p = reinterpret_cast<T*>(tab.data) + uint64_t(a.rec[uint64_t(tile + 1) * a.k].x) * tab.row_len;
+                add_to_row(p, sp, fetch(p, sp.at, tab.row_len, true), acc, scale);
             }
             __syncthreads();
-            if (w == 0) {
-#pragma unroll
-                for (int o = 0; o < 3; o++)
-#pragma unroll
-                    for (int i = 0; i < kChunk; i++) acc[i] += sum[o][lane][i];
-            }
-            __syncthreads();
         }
-        if (w == 0 && on) add_to_row(p, sp, old, acc, scale);
+        __syncthreads();                                           // (every wave has read `many`)
     }
 }
 
@@ -688,9 +744,9 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     hipError_t e = by_index(b.index_size, [&](auto iw) { return sort_records<decltype(iw)::value>(p, tab, b, w, err, s, &sorted); });
     if (e != hipSuccess) return e;
     const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), reinterpret_cast<uint32_t*>(w + p.joins),
-                       uint32_t(b.n), p.k, p.groups, p.pitch, divisor(p.chunks)};
+                       uint32_t(b.n), p.k, p.groups, p.pitch, p.lanes, divisor(p.chunks)};
     const Divisor wide = divisor((tab.row_len + 64 * kChunk - 1) / (64 * kChunk));
-    const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 2048));
+    const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 256));
     const unsigned blocks = unsigned((uint64_t(p.groups) * p.chunks * p.lanes + 255) / 256);
     return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) {
         using T = decltype(t);
@@ -710,7 +766,7 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
         };
         if (tab.row_len % kChunk == 0) by_lanes(std::true_type{});
         else by_lanes(std::false_type{});
-        hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(256), 0, s, tab, b.scale, a, wide);
+        hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(64 * kJoinWaves), 0, s, tab, b.scale, a, wide);
         return hipGetLastError();
     }); });
 }

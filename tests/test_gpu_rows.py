@@ -190,6 +190,25 @@ def test_add_large(lam, world, n, rows, width, how):
     check_close(a.local_rows(), exact, bound)
 
 
+@pytest.mark.parametrize("width", [24, 520, 1001])
+@pytest.mark.parametrize("shift", [0, 1, 5])
+def test_add_runs_at_borders(lam, world, width, shift):
+    """Runs of every length around the powers of two, so that they begin and end before, on and behind
+    any border of 8 to 64 records, runs of several borders among them."""
+    g = gen(shift)
+    lengths = [1] * shift
+    for k in (8, 16, 32, 64, 128):
+        for d in (-2, -1, 0, 1, 2):
+            lengths += [k + d, 3, 1, 2 * k + d, k]
+    rows = len(lengths)
+    i = torch.repeat_interleave(torch.arange(rows), torch.tensor(lengths))[torch.randperm(sum(lengths), generator=g)]
+    a, t = float_array(lam, world, g, rows, width, "f32")
+    v = torch.randn(i.numel(), width, generator=g).to(torch.bfloat16)
+    a.batch_add_rows(i.cuda(), v.cuda()).block()
+    exact, bound = ref.add(t, i, v)
+    check_close(a.local_rows(), exact, bound)
+
+
 @pytest.mark.parametrize("n,how", [(400, "skewed"), (30000, "skewed"), (30000, "same"), (5000, "any")])
 def test_add_repeats_its_bits(lam, world, n, how):
     g = gen(n)
