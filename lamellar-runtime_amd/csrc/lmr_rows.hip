@@ -250,6 +250,17 @@ __global__ __launch_bounds__(64) void k_rows_prefix(SortPass p) {
     p.hist[uint64_t(p.tiles) * nd + d] = sum;
 }
 
+// the lanes of the wave whose digit is this lane's
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, uint32_t bits, bool live) {
+    uint64_t same = __ballot(live);
+    for (uint32_t i = 0; i < bits; i++) {
+        const bool one = (d >> i) & 1;
+        const uint64_t m = __ballot(one);
+        same &= one ? m : ~m;
+    }
+    return same;
+}
+
 template <int IW, int IPT>
 __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatch b, RowTable tab, uint32_t* err) {
     __shared__ uint32_t cnt[kSortWaves][1 << kSortBits];
@@ -298,11 +309,7 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     for (int k = 0; k < IPT; k++) {
         const bool live = j0 + k * 64 < p.n;
         const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
-        uint64_t same = __ballot(live);
-        for (uint32_t i = 0; i < p.bits; i++) {
-            const uint64_t bit = __ballot((d >> i) & 1);
-            same &= (d >> i) & 1 ? bit : ~bit;
-        }
+        const uint64_t same = same_digit(d, p.bits, live);
         const uint32_t below = __popcll(same & ((1ull << lane) - 1));
         const uint32_t had = live ? cnt[w][d] : 0;
         rank[k] = had + below;
@@ -325,6 +332,82 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     for (int k = 0; k < IPT; k++) {
         const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
         if (j0 + k * 64 < p.n && to < p.n) p.out[to] = rec[k];     // (indices changed under way: still in bounds)
+    }
+}
+
+// Up to kOneTile records: every pass in one block and one launch, the records changing places through
+// global memory (a block's own writes, ordered by its barriers).
+constexpr uint32_t kOneTile = 8192;
+constexpr int kOneBits = 9;
+
+template <int IW>
+__global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint2* other, uint32_t passes, RowBatch b, RowTable tab, uint32_t* err) {
+    constexpr int kWaves = 16, kMost = kOneTile / 1024;
+    __shared__ uint32_t cnt[kWaves][1 << kOneBits];
+    __shared__ uint32_t wsum[kWaves];
+    const uint32_t nd = 1u << p.bits, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t rounds = (p.n + 1023) / 1024, j0 = w * rounds * 64 + lane;     // a wave's records are neighbours
+    if (threadIdx.x == 0) *p.joins = 0;
+    uint2* out = p.out;
+    for (uint32_t pass = 0; pass < passes; pass++) {
+        for (uint32_t d = lane; d < nd; d += 64) cnt[w][d] = 0;
+        uint2 rec[kMost];
+        uint32_t rank[kMost];
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            const uint32_t j = j0 + k * 64;
+            rec[k] = uint32_t(k) < rounds && j < p.n ? sort_record<IW>(p, b, tab, err, j) : uint2{kNoRow, 0};
+        }
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            if (uint32_t(k) >= rounds) break;
+            const bool live = j0 + k * 64 < p.n;
+            const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
+            const uint64_t same = same_digit(d, p.bits, live);
+            const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+            const uint32_t had = live ? cnt[w][d] : 0;
+            rank[k] = had + below;
+            __builtin_amdgcn_wave_barrier();                       // every lane has read before one writes
+            if (live && below == 0) cnt[w][d] = had + __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        uint32_t total = 0;
+        if (threadIdx.x < nd)
+#pragma unroll
+            for (int i = 0; i < kWaves; i++) total += cnt[i][threadIdx.x];
+        uint32_t run = total;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t o = __shfl_up(run, s, 64);
+            if (int(lane) >= s) run += o;
+        }
+        if (lane == 63) wsum[w] = run;
+        __syncthreads();
+        if (threadIdx.x < nd) {
+            uint32_t at = run - total;
+            for (uint32_t i = 0; i < w; i++) at += wsum[i];
+#pragma unroll
+            for (int i = 0; i < kWaves; i++) {
+                const uint32_t c = cnt[i][threadIdx.x];
+                cnt[i][threadIdx.x] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            if (uint32_t(k) >= rounds) break;
+            const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
+            if (j0 + k * 64 < p.n && to < p.n) out[to] = rec[k];
+        }
+        __threadfence_block();
+        __syncthreads();
+        p.in = out;
+        p.shift += p.bits;
+        uint2* const o = out;
+        out = other;
+        other = o;
     }
 }
 
@@ -434,7 +517,7 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
 // record): each wave, or each group of lanes that hold a short row, takes a share. The list's order is
 // no one's: every row is in it once.
 constexpr uint32_t kWaveParts = 32;
-constexpr uint32_t kJoinWaves = 16;
+constexpr uint32_t kJoinWaves = 8;
 
 __device__ __forceinline__ void add_parts(const SumArgs& a, uint32_t tile, uint32_t j0, uint32_t j1, uint32_t chunk, float (&acc)[kChunk]) {
 #pragma unroll 8
@@ -675,7 +758,7 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
 // How a batch of adds runs, and its workspace: two lists of (row, record), the digit counts, and the
 // parts of rows that reach past a group's records.
 struct AddPlan {
-    bool few;
+    bool few, one;
     uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
     uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
     uint32_t pitch;
@@ -686,7 +769,9 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     p.few = n <= kFewRecords;
     if (p.few) return p;
     const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
-    p.passes = (key_bits + kSortBits - 1) / kSortBits;
+    p.one = n <= kOneTile;
+    const uint32_t most = p.one ? kOneBits : kSortBits;
+    p.passes = (key_bits + most - 1) / most;
     p.bits = (key_bits + p.passes - 1) / p.passes;
     p.ipt = n <= 131072 ? 4 : 16;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
@@ -714,6 +799,14 @@ template <int IW>
 hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b, uint8_t* work, uint32_t* err, hipStream_t s,
                         const uint2** sorted) {
     const uint2* in = nullptr;
+    if (p.one) {
+        uint2* const a = reinterpret_cast<uint2*>(work + p.rec[0]);
+        uint2* const c = reinterpret_cast<uint2*>(work + p.rec[1]);
+        const SortPass q = {nullptr, a, nullptr, uint32_t(b.n), 0, p.bits, 1, false, reinterpret_cast<uint32_t*>(work + p.joins)};
+        hipLaunchKernelGGL((k_rows_sort_one<IW>), dim3(1), dim3(1024), 0, s, q, c, p.passes, b, tab, err);
+        *sorted = p.passes % 2 ? a : c;
+        return hipGetLastError();
+    }
     for (uint32_t i = 0; i < p.passes; i++) {
         uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
         SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 64,
@@ -746,7 +839,7 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), reinterpret_cast<uint32_t*>(w + p.joins),
                        uint32_t(b.n), p.k, p.groups, p.pitch, p.lanes, divisor(p.chunks)};
     const Divisor wide = divisor((tab.row_len + 64 * kChunk - 1) / (64 * kChunk));
-    const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 256));
+    const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 512));
     const unsigned blocks = unsigned((uint64_t(p.groups) * p.chunks * p.lanes + 255) / 256);
     return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) {
         using T = decltype(t);
