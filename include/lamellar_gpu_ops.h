@@ -501,19 +501,22 @@ lmr_status_t lmr_reduce(lmr_ctx_t* ctx, uint32_t dtype, uint32_t op, const void*
  *               `stride` elements apart; add and store also take stride 0: one row for every record.
  *               They must not overlap the table.
  * Arithmetic is f32, rounded once (to nearest, ties to even) where a narrower type is written.
- * Nothing is allocated and nothing waits; every call may be captured into a graph. Calls on one
- * table from different streams must be ordered by the caller. n <= LMR_ROW_MAX_BATCH, n * row_len <= LMR_ROW_MAX_VALUES,
+ * Nothing is allocated and nothing waits; every call may be captured into a graph. They use none of
+ * the context's workspace (only its device and error word): calls on different tables may run on
+ * several streams at once, calls that write one table must be ordered by the caller. n <= LMR_ROW_MAX_BATCH, n * row_len <= LMR_ROW_MAX_VALUES,
  * stride <= LMR_ROW_MAX_STRIDE. */
 #define LMR_ROW_MAX_LEN (1u << 18)
 #define LMR_ROWS_MAX 0xFFFFFFF0ull
 #define LMR_ROW_MAX_BATCH (1ull << 25)
 #define LMR_ROW_MAX_VALUES (1ull << 36)
 #define LMR_ROW_MAX_STRIDE 0xFFFFFFFFull
+#define LMR_ROW_SCAN 1024u
 typedef struct {
     void* data;          /* device pointer: row r starts at element r * row_len */
     float* scales;       /* 8-bit types: rows x (row_len / group) scales; otherwise unused */
-    uint32_t* claims;    /* rows words, zero before the first lmr_rows_store and left zero by each;
-                            NULL: no row occurs twice in one store */
+    uint32_t* claims;    /* rows words, zero before the first lmr_rows_store that uses them and left
+                            zero by each; used by stores of more than LMR_ROW_SCAN records, where
+                            NULL says that no row occurs twice */
     uint64_t rows;       /* <= LMR_ROWS_MAX */
     uint64_t row_len;    /* 1 .. LMR_ROW_MAX_LEN elements */
     uint32_t type;       /* lmr_row_type_t */

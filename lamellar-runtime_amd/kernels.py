@@ -468,6 +468,9 @@ class DeviceKernels:
         """The current stream as an integer (0: the default one)."""
         return torch._C._cuda_getCurrentRawStream(self.device.index or 0)
 
+    def capturing(self):
+        return torch.cuda.is_current_stream_capturing()
+
     def keep_for_stream(self, tensors):
         s = torch.cuda.current_stream(self.device)
         for t in tensors:

@@ -33,7 +33,7 @@ import torch.distributed as dist
 
 from . import _capi
 from .array import _Handle
-from .engine import index_input
+from .engine import _FORCE_EXCHANGE, index_input
 from .kernels import LamellarError, check
 from .types import DTYPES, Distribution, LmrStatus
 
@@ -54,6 +54,7 @@ ROW_TYPES = {t.name: t for t in (
     RowType("i8", 3, torch.int8, 127.0), RowType("e4m3", 4, torch.float8_e4m3fn, 448.0))}
 _BY_TORCH = {t.torch: t for t in ROW_TYPES.values()}
 MAX_ROW_LEN = 1 << 18                     # LMR_ROW_MAX_LEN
+SCAN = 1024                               # LMR_ROW_SCAN: stores of more records use claims
 _INT = (torch.int64, torch.int32)
 
 
@@ -180,9 +181,7 @@ class RowArray:
                                          int(distribution)), "lmr_layout_new")
 
     def _adopt(self, data, scales):
-        n = self.num_rows_local()
-        claims = torch.zeros(n, dtype=torch.int32, device=data.device)
-        self._table = _Table(data, scales, claims, n, self.row_len, self.rtype, self.group)
+        self._table = _Table(data.detach(), scales, None, self.num_rows_local(), self.row_len, self.rtype, self.group)
         self._streams = set()             # streams whose work may still use the tensors when the array is dropped
         self.team.barrier()
 
@@ -249,6 +248,9 @@ class RowArray:
         return RowsHandle(self, lambda: self._write(index, vals, 1.0, pad, False))
 
     # ---- one PE's part, and the exchange ----
+    def _distributed(self):
+        return self.team.num_pes() > 1 or _FORCE_EXCHANGE
+
     def _on_stream(self, k):
         """The current stream, which will use the array's memory: its reuse waits for that stream."""
         s = k.stream_id()
@@ -256,6 +258,17 @@ class RowArray:
             self._streams.add(s)
             k.keep_for_stream([t for t in (self._table.data, self._table.scales, self._table.claims) if t is not None])
         return s
+
+    def _claims(self, k, stream):
+        """The table with the words that stores of many records need: made once, but inside a capture
+        the graph gets its own (their clearing is part of the graph and has not run yet)."""
+        t = self._table
+        claims = torch.zeros(t.rows, dtype=torch.int32, device=k.device)
+        if k.capturing():
+            return _Table(t.data, t.scales, claims, t.rows, t.row_len, t.rtype, t.group)
+        t.claims, t.c.claims = claims, claims.data_ptr()
+        self._streams = {stream}          # other streams are told of it when they next use the array
+        return t
 
     def _index(self, k, index):
         """(1-D index tensor of 4 or 8 bytes, the shape it had)."""
@@ -304,7 +317,7 @@ class RowArray:
         k = self.team.kernels
         idx, shape = self._index(k, index)
         n, shape = idx.numel(), (*shape, self.row_len)
-        alone = self.team.num_pes() == 1
+        alone = not self._distributed()
         stride = self.row_len
         if out is None:
             rows = out = torch.empty(shape, dtype=rt.torch, device=k.device)
@@ -344,7 +357,7 @@ class RowArray:
         n = idx.numel()
         vals, rt = self._values(k, vals, n)
         stream = self._on_stream(k)
-        if self.team.num_pes() > 1:
+        if self._distributed():
             idx, vals, pad = self._exchange_values(k, idx, vals, pad)
             n = idx.numel()
         if n == 0:
@@ -353,7 +366,8 @@ class RowArray:
         if add:
             k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride, stream)
         else:
-            k.rows_store(self._table, idx, n, pad, vals, rt.code, stride, stream)
+            table = self._table if n <= SCAN or self._table.claims is not None else self._claims(k, stream)
+            k.rows_store(table, idx, n, pad, vals, rt.code, stride, stream)
         return None
 
     # Records travel to their rows' owner in input order (the stable pack), sources one after the

@@ -570,3 +570,56 @@ def test_decode_steps(lam, world):
         exact = ref.load(ref.codes_f64(codes, "i8"), torch.arange(len(v)), 1.0, scales, group)
         check_close(got, exact, ref.load_bound(exact, "f32", 2))
     cache.wait_all()
+
+
+def test_two_graphs_at_once(lam, world):
+    """Two captured gradients and cache writes, each with its own workspace, replayed on two streams."""
+    g = gen(21)
+    n, rows, width = 3000, 2000, 136
+    streams, graphs, sets = [torch.cuda.Stream() for _ in range(2)], [], []
+    for q in range(2):
+        t = torch.randn(rows, width, generator=g)
+        i, v = indices(g, n, rows, "skewed"), torch.randn(n, width, generator=g)
+        a, c = lam.RowArray.from_tensor(world.team(), t.cuda()), lam.RowArray(world.team(), rows, width, dtype="i8", group=17)
+        sets.append((t, i, v, a, c, i.cuda(), v.cuda()))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[q]):
+            a.batch_add_rows(sets[q][5], sets[q][6], scale=0.25).spawn()
+            c.batch_store_rows(sets[q][5], sets[q][6]).spawn()           # its first store is the captured one
+        graphs.append(graph)
+    for _ in range(3):
+        for q in range(2):
+            with torch.cuda.stream(streams[q]):
+                graphs[q].replay()
+    torch.cuda.synchronize()
+    for t, i, v, a, c, _, _ in sets:
+        now, total = t, 0.0                               # three calls' bounds, and this side's rounding between
+        for _ in range(3):
+            exact, bound = ref.add(now, i, v, 0.25)
+            now, total = exact.float(), total + bound + exact.abs() * ref.U32
+        check_close(a.local_rows(), exact, total)
+        last = ref.last_records(i, rows)
+        at, rec = torch.tensor(list(last)), torch.tensor([last[r] for r in last])
+        codes, scales = ref.quantise(v[rec], "i8", 17)
+        assert torch.equal(c.local_scales().cpu()[at], scales)
+        assert torch.equal(c.local_rows().cpu()[at].view(torch.uint8), codes)
+    world.wait_all()
+
+
+def test_batches_past_32_bits(lam, world):
+    """Values and results of more than 2^32 elements."""
+    n, width, rows = 70000, 65536, 10
+    t = torch.arange(rows * 4).view(rows, 4).float().repeat(1, width // 4).to(torch.bfloat16)
+    a = lam.RowArray.from_tensor(world.team(), t.cuda())
+    i = torch.arange(n, device="cuda") % rows
+    got = a.batch_load_rows(i).spawn().value()
+    for k in (0, 65535, 65536, n - 11, n - 1):
+        assert torch.equal(got[k].cpu(), t[k % rows]), k
+    s = lam.RowArray(world.team(), rows, width)
+    s.batch_add_rows(i, got).block()
+    assert torch.equal(s.local_rows().cpu(), t.float() * (n // rows))     # whole numbers below 2^24
+    q = lam.RowArray(world.team(), rows, width, dtype="i8", group=64)
+    got[-1].fill_(1.0)
+    q.batch_store_rows(i, got).block()
+    assert torch.equal(q.batch_load_rows([rows - 1], out_dtype="f32").block().cpu(), torch.ones(1, width))

@@ -24,6 +24,9 @@ class CpuRowKernels(CpuTestKernels):
     def keep_for_stream(self, tensors):
         pass
 
+    def capturing(self):
+        return False
+
     def pack(self, layout, gidx, n, vals, dt, iw, stable=True, want_pos=True):
         ok = (gidx >= 0) & (gidx < layout.size)          # out of bounds: reported and dropped
         if not bool(ok.all()):
