@@ -550,10 +550,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, flo
                 hi = min(hi, next + step);
                 lo = next;
             }
-            parts = lo - tile + 1;
+            parts = row < uint32_t(tab.rows) ? lo - tile + 1 : 0;  // (see k_rows_sum: changed indices)
             const uint32_t chunk = (item - which * wide.d) * 64 + lane;
             const Span sp = span_of(chunk, tab.row_len);
-            if (parts <= kWaveParts && sp.lo < sp.hi) {
+            if (parts > 0 && parts <= kWaveParts && sp.lo < sp.hi) {
                 T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len;
                 const Chunk<T> old = fetch(p, sp.at, tab.row_len, true);
                 float acc[kChunk] = {};
@@ -773,7 +773,7 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     const uint32_t most = p.one ? kOneBits : kSortBits;
     p.passes = (key_bits + most - 1) / most;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    p.ipt = n <= 262144 ? 4 : 16;
+    p.ipt = n <= 65536 ? 2 : n <= 262144 ? 4 : 16;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
@@ -811,11 +811,15 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
         uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
         SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 128,
                       reinterpret_cast<uint32_t*>(work + p.joins)};
-        if (p.ipt == 4) hipLaunchKernelGGL((k_rows_count<IW, 4>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
-        else hipLaunchKernelGGL((k_rows_count<IW, 16>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
-        if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
-        if (p.ipt == 4) hipLaunchKernelGGL((k_rows_place<IW, 4>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
-        else hipLaunchKernelGGL((k_rows_place<IW, 16>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        auto go = [&](auto ipt) {
+            constexpr int IPT = decltype(ipt)::value;
+            hipLaunchKernelGGL((k_rows_count<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+            if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
+            hipLaunchKernelGGL((k_rows_place<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+        };
+        if (p.ipt == 2) go(std::integral_constant<int, 2>{});
+        else if (p.ipt == 4) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 16>{});
         in = out;
     }
     *sorted = in;
