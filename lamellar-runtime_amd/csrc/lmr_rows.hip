@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
 
 // Up to kOneTile records: every pass in one block and one launch, the records changing places through
 // global memory (a block's own writes, ordered by its barriers).
-constexpr uint32_t kOneTile = 8192;
+constexpr uint32_t kOneTile = 6144;
 constexpr int kOneBits = 9;
 
 template <int IW>
@@ -635,40 +635,43 @@ __device__ __forceinline__ Chunk<T> pack_codes(const float (&v)[kChunk], const G
     return {{to_codes<T>(v, q), to_codes<T>(v + 4, q)}};
 }
 
-// WPR waves per record (1: four records a block). Groups of up to 512 elements: as many lanes as hold
-// one (a power of two) find its largest |x| by shuffles and keep its values in registers. Longer
-// groups are read twice, the second time from cache.
-template <typename T, typename V, int IW, int WPR>
+// L lanes per record: 8 to 64 (as many as hold a short row, so that a wave takes several), or the whole
+// block. Groups of up to 512 elements: as many lanes as hold one (a power of two) find its largest |x|
+// by shuffles and keep its values in registers. Longer groups are read twice, the second time from cache.
+template <typename T, typename V, int IW, int L>
 __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, const V* vals, uint32_t* err, int how, uint32_t lpg) {
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, part = WPR == 4 ? w : 0;
-    uint64_t t = WPR == 4 ? blockIdx.x : uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(w);
+    constexpr int kWaves = L > 64 ? L / 64 : 1;                    // waves that share a record
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, mine_of = threadIdx.x % L;
+    uint32_t t = blockIdx.x * (256 / L) + threadIdx.x / L;
+    if constexpr (L >= 64) t = __builtin_amdgcn_readfirstlane(t);
     if (t >= b.n) return;
-    const int64_t r = row_of<IW>(b, t, tab.rows, err, lane == 0);
+    const int64_t r = row_of<IW>(b, t, tab.rows, err, mine_of == 0);
     bool mine = r >= 0;
     if (how == kScanned) {
         bool later = false;
-        for (uint64_t u = t + 1 + lane; u < b.n; u += 64) later |= row_index<IW>(b, u) == r;
-        mine = mine && !__ballot(later);
+        for (uint32_t u = t + 1 + (L > 64 ? lane : mine_of); u < b.n; u += L > 64 ? 64 : L) later |= row_index<IW>(b, u) == r;
+        const uint64_t found = __ballot(later);
+        mine = mine && !(L >= 64 ? found : found >> (lane & ~uint32_t(L - 1)) & ((1ull << (L & 63)) - 1));
     } else if (how == kClaimed) {
-        mine = mine && tab.claims[r] == uint32_t(t) + 1;
-        if constexpr (WPR > 1) __syncthreads();                    // every wave has read the claim
-        if (mine && part == 0 && lane == 0) tab.claims[r] = 0;
+        mine = mine && tab.claims[r] == t + 1;
+        if constexpr (kWaves > 1) __syncthreads();                 // every wave has read the claim
+        if (mine && mine_of == 0) tab.claims[r] = 0;
     }
     if (!mine) return;
     T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
-    const V* x = vals + t * b.stride;
+    const V* x = vals + uint64_t(t) * b.stride;
     if constexpr (!is_code<T>::v) {
 #pragma unroll 4
-        for (uint32_t c = part * 64 + lane; c * kChunk < tab.row_len; c += WPR * 64) {
+        for (uint32_t c = mine_of; c * kChunk < tab.row_len; c += L) {
             const uint32_t at = span_of(c, tab.row_len).at;
             float v[kChunk];
             unpack(fetch(x, at, tab.row_len, true), v);
             put(row, at, tab.row_len, pack<T>(v));
         }
     } else if (lpg) {
-        const uint32_t per = 64 / lpg, in = lane & (lpg - 1), at = span_of(in, tab.group).at;
-        for (uint32_t g0 = part * per; g0 < tab.groups; g0 += WPR * per) {
-            const uint32_t g = g0 + lane / lpg;
+        const uint32_t in = mine_of & (lpg - 1), at = span_of(in, tab.group).at;
+        for (uint32_t g0 = 0; g0 < tab.groups; g0 += L / lpg) {
+            const uint32_t g = g0 + mine_of / lpg;
             const bool on = g < tab.groups && in * kChunk < tab.group;
             float v[kChunk];
             unpack(fetch(x + g * tab.group, at, tab.group, on), v);
@@ -677,37 +680,38 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
             put(row + g * tab.group, at, tab.group, pack_codes<T>(v, q));
             if (in == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
-    } else {
+    } else if constexpr (L >= 64) {
         __shared__ uint32_t top[2][4];
         for (uint32_t g = 0; g < tab.groups; g++) {
             const V* xg = x + uint64_t(g) * tab.group;
             T* rg = row + uint64_t(g) * tab.group;
             uint32_t m = 0;
 #pragma unroll 4
-            for (uint32_t c = part * 64 + lane; c * kChunk < tab.group; c += WPR * 64) {
+            for (uint32_t c = mine_of; c * kChunk < tab.group; c += L) {
                 float v[kChunk];
                 unpack(fetch(xg, span_of(c, tab.group).at, tab.group, true), v);
                 m = max(m, max_bits(v));
             }
             m = max_over(m, 64);
-            if constexpr (WPR > 1) {                               // (two sets: a wave may be one group ahead)
+            if constexpr (kWaves > 1) {                            // (two sets: a wave may be one group ahead)
                 if (lane == 0) top[g & 1][w] = m;
                 __syncthreads();
                 m = max(max(top[g & 1][0], top[g & 1][1]), max(top[g & 1][2], top[g & 1][3]));
             }
             const GroupScale q = group_scale<T>(m);
 #pragma unroll 4
-            for (uint32_t c = part * 64 + lane; c * kChunk < tab.group; c += WPR * 64) {
+            for (uint32_t c = mine_of; c * kChunk < tab.group; c += L) {
                 const uint32_t at = span_of(c, tab.group).at;
                 float v[kChunk];
                 unpack(fetch(xg, at, tab.group, true), v);
                 put(rg, at, tab.group, pack_codes<T>(v, q));
             }
-            if (part == 0 && lane == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
+            if (mine_of == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
     }
 }
 
+bool is_float_type(uint32_t type) { return type <= LMR_ROW_BF16; }
 template <typename F>
 hipError_t by_value_type(uint32_t type, F&& f) {
     switch (type) {
@@ -773,7 +777,7 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     const uint32_t most = p.one ? kOneBits : kSortBits;
     p.passes = (key_bits + most - 1) / most;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    p.ipt = n <= 65536 ? 2 : n <= 262144 ? 4 : 16;
+    p.ipt = n <= 16384 ? 1 : n <= 65536 ? 2 : n <= 262144 ? 4 : 16;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
@@ -817,7 +821,8 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
             if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
             hipLaunchKernelGGL((k_rows_place<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
         };
-        if (p.ipt == 2) go(std::integral_constant<int, 2>{});
+        if (p.ipt == 1) go(std::integral_constant<int, 1>{});
+        else if (p.ipt == 2) go(std::integral_constant<int, 2>{});
         else if (p.ipt == 4) go(std::integral_constant<int, 4>{});
         else go(std::integral_constant<int, 16>{});
         in = out;
@@ -872,17 +877,28 @@ hipError_t launch_store(const RowTable& tab, const RowBatch& b, const void* vals
     uint32_t lpg = 0;                                              // lanes that hold a group, 0: longer groups
     if (tab.group <= 64 * kChunk)
         for (lpg = 1; lpg * kChunk < tab.group;) lpg *= 2;
-    // four waves share a record where records alone do not fill the card and a row has work for them
-    // (64 rows of 4096: 3.5 us against 7.0 with one wave; 2048 rows of 1024: 6.6 against 6.3)
-    const bool wide = b.n < 2048 && tab.row_len > 512;
+    // a block shares a record where records alone do not fill the card and a row has work for it (64
+    // rows of 4096: 3.5 us against 7.0 with a wave; 2048 rows of 1024: 6.6 against 6.3)
+    const uint32_t need = lpg ? std::min(64u, lpg * tab.groups) : 64u, held = is_float_type(tab.type) ? (tab.row_len + 7) / 8 : need;
+    const uint32_t lanes = b.n < 2048 && tab.row_len > 512 ? 256 : held > 32 ? 64 : held > 16 ? 32 : held > 8 ? 16 : 8;
     return by_row_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
         using T = decltype(t);
         using V = decltype(v);
         constexpr int IW = decltype(iw)::value;
         const V* x = reinterpret_cast<const V*>(vals);
         if (how == kClaimed) hipLaunchKernelGGL((k_rows_claim<IW>), dim3(unsigned((b.n + 255) / 256)), dim3(256), 0, s, tab, b, err);
-        if (wide) hipLaunchKernelGGL((k_rows_store<T, V, IW, 4>), dim3(unsigned(b.n)), dim3(256), 0, s, tab, b, x, err, how, lpg);
-        else hipLaunchKernelGGL((k_rows_store<T, V, IW, 1>), dim3(unsigned((b.n + 3) / 4)), dim3(256), 0, s, tab, b, x, err, how, lpg);
+        auto go = [&](auto l) {
+            constexpr int L = decltype(l)::value;
+            hipLaunchKernelGGL((k_rows_store<T, V, IW, L>), dim3(unsigned((b.n + 256 / L - 1) / (256 / L))), dim3(256), 0, s, tab, b, x,
+                               err, how, lpg);
+        };
+        switch (lanes) {
+        case 8: go(std::integral_constant<int, 8>{}); break;
+        case 16: go(std::integral_constant<int, 16>{}); break;
+        case 32: go(std::integral_constant<int, 32>{}); break;
+        case 64: go(std::integral_constant<int, 64>{}); break;
+        default: go(std::integral_constant<int, 256>{});
+        }
         return hipGetLastError();
     }); }); });
 }

@@ -227,6 +227,8 @@ class RowArray:
         a tensor to write instead of a new one; its rows may be strided."""
         scale, pad = _scale(scale), _pad(pad)
         if out is not None:
+            if not isinstance(out, torch.Tensor):
+                raise LamellarError(LmrStatus.INVALID, f"out is a tensor, not {type(out).__name__}")
             rt = _value_type(out.dtype)
             if out_dtype is not None and _value_type(out_dtype) is not rt:
                 raise LamellarError(LmrStatus.INVALID, f"out is {rt.name}, not {out_dtype}")

@@ -190,6 +190,38 @@ def test_add_large(lam, world, n, rows, width, how):
     check_close(a.local_rows(), exact, bound)
 
 
+@pytest.mark.parametrize("n", [700, 6144, 6145, 20000])
+@pytest.mark.parametrize("rows", [3, 511, 512, (1 << 18) - 1, 1 << 18, (1 << 20) + 7, (1 << 27) + 3])
+def test_add_key_widths(lam, world, n, rows):
+    """Tables of few to many rows: one to four sort passes, indices at both ends."""
+    g = gen(n)
+    a = lam.RowArray(world.team(), rows, 1, dtype="f16")
+    i = torch.randint(rows, (n,), generator=g)
+    i[: n // 4] = rows - 1 - torch.randint(min(rows, 40), (n // 4,), generator=g)
+    i[-3:] = 0
+    v = torch.randint(-4, 5, (n, 1), generator=g).to(torch.float16)       # every sum exact, below 2^11
+    a.batch_add_rows(i.cuda(), v.cuda()).block()
+    at, back = torch.unique(i, return_inverse=True)
+    exact = torch.zeros(len(at), 1, dtype=torch.float64).index_add_(0, back, v.double())
+    fits = exact.abs() <= 2048                                            # (3 rows: some sums are larger and round)
+    got = a.batch_load_rows(at.cuda(), out_dtype="f32").block().cpu().double()
+    assert torch.equal(got[fits], exact[fits])
+    assert ((got - exact).abs() <= exact.abs() * ref.u("f16")).all()
+    assert int((a.local_rows() != 0).sum()) == int((exact != 0).sum())
+
+
+def test_add_very_many(lam, world):
+    """More tiles than one launch adds up by itself (the sort's prefix launch)."""
+    n, rows, width = 1200007, 5000, 8
+    g = gen(n)
+    a, t = float_array(lam, world, g, rows, width, "f32")
+    i = indices(g, n, rows, "skewed")
+    v = torch.randn(n, width, generator=g).to(torch.bfloat16)
+    a.batch_add_rows(i.cuda(), v.cuda(), scale=0.5).block()
+    exact, bound = ref.add(t, i, v, 0.5)
+    check_close(a.local_rows(), exact, bound)
+
+
 @pytest.mark.parametrize("width", [24, 520, 1001])
 @pytest.mark.parametrize("shift", [0, 1, 5])
 def test_add_runs_at_borders(lam, world, width, shift):
@@ -322,7 +354,8 @@ def test_gradient_by_differences(lam, world):
 @pytest.mark.parametrize("kind", CODES)
 @pytest.mark.parametrize("n,rows,width,group", [(1, 1, 1, 1), (4, 9, 30, 3), (64, 100, 1024, 128), (65, 300, 640, 80), (200, 4000, 96, 32),
                                                 (3000, 5000, 256, 64), (5, 6, 4097, 4097), (37, 50, 1200, 600), (2000, 2000, 1000, 100),
-                                                (10, 30, 8192, 512), (1030, 2048, 192, 192)])
+                                                (10, 30, 8192, 512), (1030, 2048, 192, 192), (2600, 2600, 16, 8), (999, 1000, 7, 7),
+                                                (2049, 2100, 130, 26), (3, 3, 1500, 500), (2050, 2100, 1100, 1100)])
 def test_store_codes(lam, world, kind, vals, n, rows, width, group):
     g = gen(n + width)
     a = lam.RowArray(world.team(), rows, width, dtype=kind, group=group)

@@ -130,6 +130,7 @@ def test_refused_batches(lam, team):
     refused(lam, UNSUPPORTED, a.batch_load_rows, [0], out_dtype="i8")
     refused(lam, UNSUPPORTED, a.batch_load_rows, [0], out=torch.empty(1, 6, dtype=torch.int32))
     refused(lam, INVALID, a.batch_load_rows, [0], out=torch.empty(1, 6), out_dtype="bf16")
+    refused(lam, INVALID, a.batch_load_rows, [0], out=np.empty((1, 6)))
     mem = torch.empty(100)
     for out, status in [(torch.empty(2, 6), LENGTH), (torch.empty(18), LENGTH), (torch.empty(6, 3).t(), INVALID),
                         (mem.as_strided((3, 6), (4, 1)), INVALID), (mem.as_strided((3, 6), (0, 1)), INVALID),
@@ -156,6 +157,12 @@ def test_one_pe_batches(lam, team):
     h = a.batch_load_rows([2])
     assert h.value() is h.spawn().value() is h.block()
     assert a.batch_add_rows([], torch.ones(0, 4)).block() is None
+    assert a.batch_add_rows([], torch.ones(4)).block() is None
+    assert a.batch_load_rows(np.int64(2)).block().shape == (4,)
+    weight = torch.nn.Parameter(torch.ones(3, 4))        # a parameter's memory, its gradient left alone
+    p = lam.RowArray.from_tensor(team, weight)
+    p.batch_add_rows([2], torch.ones(4, requires_grad=True), scale=2).block()
+    assert weight[2].tolist() == [3, 3, 3, 3] and not p.local_rows().requires_grad
 
 
 def test_c_entry_refusals(capi, lam):
