@@ -970,6 +970,7 @@ struct OnDevice {
     explicit OnDevice(int device) {
         ok = hipGetDevice(&was) == hipSuccess;
         if (ok && was != device) ok = moved = hipSetDevice(device) == hipSuccess;
+        (void)hipGetLastError();                             // what an earlier call left is not this one's
     }
     ~OnDevice() { if (moved) (void)hipSetDevice(was); }
 };

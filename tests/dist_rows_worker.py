@@ -1,4 +1,4 @@
-"""One PE of the row batches over several PEs (test_gpu_dist_rows.py): every PE shares the box's GPU.
+"""One PE of the row batches over several PEs (test_batch_rows_pes.py): every PE shares the box's GPU.
 
 Runs lookups, adds and stores whose rows collide across PEs through RowArray's exchange and the HIP
 kernels of every owner, and saves this PE's records and results."""

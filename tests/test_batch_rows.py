@@ -219,7 +219,7 @@ def _worker(rank, ws, port, outdir, dist_kind):
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(ws), LOCAL_RANK=str(rank))
     from _lamellar_bootstrap import load_package
     lam = load_package()
-    from test_rows import CpuRowKernels, _inputs
+    from test_batch_rows import CpuRowKernels, _inputs
     world = lam.LamellarWorldBuilder().with_kernels(CpuRowKernels).build()
     team, res = world.team(), {}
     rows, width = 23, 6
