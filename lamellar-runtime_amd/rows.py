@@ -17,9 +17,15 @@ batch depends on its arguments alone: the records of a row are added in an order
 indices, and of several records stored to one row the last one of the batch stands, on the highest
 PE that names the row when several do.
 
+Indices are integers of any shape: torch tensors (int32 and int64 are read as they are), numpy arrays,
+lists, one number. Values are torch tensors of f32, f16 or bf16; host sequences are taken as f32. A
+batch has at most 2^25 records and 2^36 elements.
+
 Handles are lazy, as the element arrays': spawn() enqueues the batch on torch's current stream,
 value() gives its result for work ordered after it on that stream, block() waits and raises what the
-batch found wrong. With several PEs every batch is collective: all PEs issue the same sequence of
+batch found wrong. A spawned batch reads its inputs in stream order, so later work on the stream may
+change them; batches that write one array are ordered by the caller if they use several streams. At one
+PE a batch may be captured into a graph; each graph has its own workspace. With several PEs every batch is collective: all PEs issue the same sequence of
 batches (an empty one where a PE has nothing to send).
 """
 from __future__ import annotations
@@ -33,7 +39,7 @@ import torch.distributed as dist
 
 from . import _capi
 from .array import _Handle
-from .engine import _FORCE_EXCHANGE, index_input
+from .engine import _FORCE_EXCHANGE, Owned, index_input
 from .kernels import LamellarError, check
 from .types import DTYPES, Distribution, LmrStatus
 
@@ -54,6 +60,7 @@ ROW_TYPES = {t.name: t for t in (
     RowType("i8", 3, torch.int8, 127.0), RowType("e4m3", 4, torch.float8_e4m3fn, 448.0))}
 _BY_TORCH = {t.torch: t for t in ROW_TYPES.values()}
 MAX_ROW_LEN = 1 << 18                     # LMR_ROW_MAX_LEN
+MAX_ROWS = 0xFFFFFFF0                     # LMR_ROWS_MAX, of one PE
 SCAN = 1024                               # LMR_ROW_SCAN: stores of more records use claims
 _INT = (torch.int64, torch.int32)
 
@@ -179,6 +186,8 @@ class RowArray:
         self.layout = _capi.lmr_layout_t()
         check(_capi.lib().lmr_layout_new(ctypes.byref(self.layout), rows, team.num_pes(), team.my_pe(),
                                          int(distribution)), "lmr_layout_new")
+        if self.num_rows_local() > MAX_ROWS:
+            raise LamellarError(LmrStatus.INVALID, f"{self.num_rows_local()} rows on one PE (at most {MAX_ROWS})")
 
     def _adopt(self, data, scales):
         self._table = _Table(data.detach(), scales, None, self.num_rows_local(), self.row_len, self.rtype, self.group)
@@ -274,6 +283,8 @@ class RowArray:
 
     def _index(self, k, index):
         """(1-D index tensor of 4 or 8 bytes, the shape it had)."""
+        if isinstance(index, Owned):
+            index = index.value
         if isinstance(index, torch.Tensor):
             shape = index.shape
             if index.dtype in _INT and index.device == k.device:
@@ -291,7 +302,9 @@ class RowArray:
         return index_input(k, a.reshape(-1))[1], torch.Size(a.shape)
 
     def _values(self, k, vals, n):
-        """(n x row_len tensor whose rows are contiguous, elements between them)."""
+        """(n x row_len tensor whose rows are contiguous, their type)."""
+        if isinstance(vals, Owned):
+            vals = vals.value
         if not isinstance(vals, torch.Tensor):
             vals = torch.from_numpy(np.ascontiguousarray(np.asarray(vals), dtype=np.float32))
         rt = _value_type(vals.dtype)

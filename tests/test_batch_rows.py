@@ -107,6 +107,9 @@ def test_refused_arrays(lam, team):
     a = F(team, codes, scales=torch.ones(4, 2))
     assert (a.dtype, a.group, len(a), a.row_len) == ("i8", 3, 4, 6) and a.local_rows().data_ptr() == codes.data_ptr()
     assert R.new(team, 3, 5, dtype="e4m3").block().group == 5
+    e = F(team, torch.ones(4, 6).to(torch.float8_e4m3fn), scales=torch.ones(4, 1))
+    assert e.dtype == "e4m3" and e.batch_load_rows([1]).block().dtype == torch.bfloat16
+    refused(lam, INVALID, R._set_up, object.__new__(R), team, 0xFFFFFFF1, 1, lam.Distribution.Block, lam.ROW_TYPES["i8"], 1)
 
 
 def test_refused_batches(lam, team):
@@ -154,6 +157,8 @@ def test_one_pe_batches(lam, team):
     assert a.batch_load_rows(1, out_dtype="f32").block().tolist() == [8, 9, 10, 11]
     a.batch_add_rows([[1], [1]], torch.ones(4), scale=0.5).block()
     assert a.batch_load_rows([[1, -1]], pad=-1).block().tolist() == [[[9, 10, 11, 12], [0, 0, 0, 0]]]
+    a.batch_store_rows(lam.Owned(torch.tensor([4])), lam.Owned(torch.ones(1, 4))).block()
+    assert a.batch_load_rows(lam.Owned([4])).block().tolist() == [[1, 1, 1, 1]]
     h = a.batch_load_rows([2])
     assert h.value() is h.spawn().value() is h.block()
     assert a.batch_add_rows([], torch.ones(0, 4)).block() is None

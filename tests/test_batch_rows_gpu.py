@@ -640,6 +640,30 @@ def test_two_graphs_at_once(lam, world):
     world.wait_all()
 
 
+@pytest.mark.parametrize("width", [1 << 18, (1 << 18) - 1, (1 << 18) - 8])
+def test_longest_rows(lam, world, width):
+    g = gen(width)
+    for n in (5, 700):
+        rows = 6
+        a, t = float_array(lam, world, g, rows, width, "bf16")
+        i = indices(g, n, rows, "any")
+        got = a.batch_load_rows(i.cuda(), out_dtype="f32").block()
+        assert torch.equal(got.cpu()[[0, n - 1]], t[i[[0, n - 1]]].float())
+        s = lam.RowArray(world.team(), rows, width)
+        s.batch_add_rows(i.cuda(), torch.ones(width, device="cuda")).block()
+        assert torch.equal(s.local_rows().cpu(), torch.bincount(i, minlength=rows).float()[:, None].expand(rows, width))
+    for group in (width, 4 if width % 4 == 0 else 3):
+        if width % group:
+            continue
+        q = lam.RowArray(world.team(), rows, width, dtype="i8", group=group)
+        q.batch_store_rows([3, 0], t[:2].cuda()).block()
+        codes, scales = ref.quantise(t[:2], "i8", group)
+        assert torch.equal(q.local_scales().cpu()[[3, 0]], scales)
+        assert torch.equal(q.local_rows().cpu()[[3, 0]].view(torch.uint8), codes)
+        exact = ref.load(ref.codes_f64(codes, "i8"), torch.tensor([1, 0]), 1.0, scales, group)
+        check_close(q.batch_load_rows([0, 3], out_dtype="f32").block(), exact, ref.load_bound(exact, "f32", 2))
+
+
 def test_batches_past_32_bits(lam, world):
     """Values and results of more than 2^32 elements."""
     n, width, rows = 70000, 65536, 10
