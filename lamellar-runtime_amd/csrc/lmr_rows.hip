@@ -437,10 +437,10 @@ struct SumArgs {
     Divisor chunks;       // column chunks of `lanes` * 8
 };
 
-// (WHOLE: rows of a multiple of 8 elements, whose chunks do not overlap)
-template <typename T, typename V, int LPR, bool WHOLE>
+// (WHOLE: rows of a multiple of 8 elements, whose chunks do not overlap. U: records whose values are in
+// flight together)
+template <typename T, typename V, int LPR, bool WHOLE, int U>
 __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, const V* vals, SumArgs a) {
-    constexpr int U = WHOLE ? 8 : 4;                               // records whose values are in flight together
     constexpr bool kLong = WHOLE || LPR > 8;                       // (shorter rows take the fewest lanes)
     uint32_t gid = (blockIdx.x * 256u + threadIdx.x) / LPR;
     if constexpr (LPR == 64) gid = __builtin_amdgcn_readfirstlane(gid);
@@ -798,10 +798,10 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
     p.chunks = (cols + p.lanes - 1) / p.lanes;
     // 32 records a group, fewer where that would leave less than about 8 waves per compute unit (131072
-    // records of 4096, all launches: 564, 519, 510, 505 us with 8, 16, 24, 32; 5003 of 1001: 40.7, 47, 55,
-    // 61)
+    // records of 4096, all launches: 564, 519, 510, 505 us with 8, 16, 24, 32; 5003 of 1001: 34.4, 36.9, 43
+    // us with 4, 8, 16)
     const uint64_t waves = n * p.chunks * p.lanes / 64;
-    p.k = waves >= 32 * 2048 ? 32 : waves >= 16 * 2048 ? 16 : 8;
+    p.k = waves >= 32 * 2048 ? 32 : waves >= 16 * 2048 ? 16 : waves >= 8 * 2048 ? 8 : 4;
     p.groups = uint32_t((n + p.k - 1) / p.k);
     p.pitch = cols * kChunk;
     uint64_t at = 0;
@@ -871,20 +871,22 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
         using T = decltype(t);
         using V = decltype(v);
         const V* x = reinterpret_cast<const V*>(vals);
-        auto sum = [&](auto lanes, auto whole) {
-            hipLaunchKernelGGL((k_rows_sum<T, V, decltype(lanes)::value, decltype(whole)::value>), dim3(blocks), dim3(256), 0, s,
-                               tab, b, x, a);
+        auto sum = [&](auto lanes, auto whole, auto u) {
+            hipLaunchKernelGGL((k_rows_sum<T, V, decltype(lanes)::value, decltype(whole)::value, decltype(u)::value>), dim3(blocks),
+                               dim3(256), 0, s, tab, b, x, a);
         };
-        auto by_lanes = [&](auto whole) {
+        auto by_lanes = [&](auto whole, auto u) {
             switch (p.lanes) {
-            case 8: sum(std::integral_constant<int, 8>{}, whole); break;
-            case 16: sum(std::integral_constant<int, 16>{}, whole); break;
-            case 32: sum(std::integral_constant<int, 32>{}, whole); break;
-            default: sum(std::integral_constant<int, 64>{}, whole);
+            case 8: sum(std::integral_constant<int, 8>{}, whole, u); break;
+            case 16: sum(std::integral_constant<int, 16>{}, whole, u); break;
+            case 32: sum(std::integral_constant<int, 32>{}, whole, u); break;
+            default: sum(std::integral_constant<int, 64>{}, whole, u);
             }
         };
-        if (tab.row_len % kChunk == 0) by_lanes(std::true_type{});
-        else by_lanes(std::false_type{});
+        // (131072 bf16 records of 4096: 512 us with 4 in flight, 502 with 8; 5003 of 1001: 36.8 and 38.4)
+        if (tab.row_len % kChunk) by_lanes(std::false_type{}, std::integral_constant<int, 4>{});
+        else if (p.k == 4) by_lanes(std::true_type{}, std::integral_constant<int, 4>{});
+        else by_lanes(std::true_type{}, std::integral_constant<int, 8>{});
         hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(64 * kJoinWaves), 0, s, tab, b.scale, a, wide);
         return hipGetLastError();
     }); });
