@@ -433,8 +433,9 @@ struct SumArgs {
     float* first;         // [tiles][pitch]
     float* last;
     uint32_t* joins;      // [0]: rows to join, [1 ..]: the tiles in which they begin, in any order
-    uint32_t n, k, tiles, pitch, lanes;
-    Divisor chunks;       // column chunks of `lanes` * 8
+    uint32_t n, k, tiles, pitch;
+    uint32_t lanes;       // of a row's part in k_rows_join
+    Divisor chunks;       // column chunks of k_rows_sum
 };
 
 // (WHOLE: rows of a multiple of 8 elements, whose chunks do not overlap. U: records whose values are in
@@ -525,11 +526,13 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
     if (open && on) store_chunk(began ? first : last, pack<float>(acc));
 }
 
-// Rows that reach past the tile after the one in which they begin: a wave takes such a row and 512
-// columns and adds its parts in order. Where there are many parts the block does it together (one row may
-// have every record: 131072 records of 4096 then take 368 us in all): each wave, or each group of lanes
-// that hold a short row, takes a share. The list's order is no one's: every row is in it once.
-constexpr uint32_t kWaveParts = 32;
+// Rows that reach past the tile after the one in which they begin: a wave takes such a row and the columns
+// that `lanes` lanes hold, its lane groups a share of the parts each. Where there are many parts (one row
+// may have every record) the block does it together. Few lanes, so that the parts of one row are read by
+// as many compute units as its columns allow (8192 records of 512 columns, all of one row: 64, 45, 35 us
+// with 64, 32, 16 lanes; 131072 of 4096 as tokens come: 502, 502, 506). The list's order is no one's:
+// every row is in it once, and its parts are added in an order that their number fixes.
+constexpr uint32_t kWaveParts = 64;
 constexpr uint32_t kJoinWaves = 8;
 
 __device__ __forceinline__ void add_parts(const SumArgs& a, uint32_t tile, uint32_t j0, uint32_t j1, uint32_t chunk, float (&acc)[kChunk]) {
@@ -548,6 +551,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, flo
     __shared__ float sum[kJoinWaves][64][kChunk + 1];
     __shared__ uint32_t many[kJoinWaves];
     const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), items = *a.joins * wide.d, gap = gridDim.x;
+    const uint32_t per = 64 / a.lanes, group = lane / a.lanes;     // shares of a wave, this lane's
     for (uint32_t base = blockIdx.x; base < items; base += gap * kJoinWaves) {
         const uint32_t item = base + gap * w;                      // neighbours go to different blocks
         uint32_t parts = 0;
@@ -564,14 +568,22 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, flo
                 lo = next;
             }
             parts = row < uint32_t(tab.rows) ? lo - tile + 1 : 0;  // (see k_rows_sum: changed indices)
-            const uint32_t chunk = (item - which * wide.d) * 64 + lane;
+            const uint32_t chunk = (item - which * wide.d) * a.lanes + lane % a.lanes;
             const Span sp = span_of(chunk, tab.row_len);
-            if (parts > 0 && parts <= kWaveParts && sp.lo < sp.hi) {
+            if (parts > 0 && parts <= kWaveParts) {
                 T* p = reinterpret_cast<T*>(tab.data) + uint64_t(row) * tab.row_len;
-                const Chunk<T> old = fetch(p, sp.at, tab.row_len, true);
+                const bool on = sp.lo < sp.hi;
+                const Chunk<T> old = fetch(p, sp.at, tab.row_len, on && group == 0);
+                const uint32_t share = (parts + per - 1) / per;
                 float acc[kChunk] = {};
-                add_parts(a, tile, 0, parts, chunk, acc);
-                add_to_row(p, sp, old, acc, scale);
+                if (on) add_parts(a, tile, min(parts, group * share), min(parts, (group + 1) * share), chunk, acc);
+                for (uint32_t o = 1; o < per; o++)
+#pragma unroll
+                    for (int i = 0; i < kChunk; i++) {
+                        const float v = __shfl(acc[i], int(o * a.lanes + lane % a.lanes), 64);
+                        if (group == 0) acc[i] += v;
+                    }
+                if (on && group == 0) add_to_row(p, sp, old, acc, scale);
             }
         }
         if (lane == 0) many[w] = parts > kWaveParts ? parts : 0;
@@ -580,8 +592,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, flo
             const uint32_t n = many[i];                            // (alike in the whole block)
             if (n == 0) continue;
             const uint32_t which = uint32_t(quotient64(base + gap * i, wide)), tile = a.joins[1 + which];
-            const uint32_t per = 64 / a.lanes, mine = w * per + lane / a.lanes, share = (n + kJoinWaves * per - 1) / (kJoinWaves * per);
-            const uint32_t chunk = (base + gap * i - which * wide.d) * 64 + lane % a.lanes;
+            const uint32_t mine = w * per + group, share = (n + kJoinWaves * per - 1) / (kJoinWaves * per);
+            const uint32_t chunk = (base + gap * i - which * wide.d) * a.lanes + lane % a.lanes;
             const Span sp = span_of(chunk, tab.row_len);
             const bool on = sp.lo < sp.hi;
             float acc[kChunk] = {};
@@ -589,7 +601,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_rows_join(RowTable tab, flo
 #pragma unroll
             for (int k = 0; k < kChunk; k++) sum[w][lane][k] = acc[k];
             __syncthreads();
-            if (w == 0 && lane < a.lanes && on) {
+            if (w == 0 && group == 0 && on) {
                 for (uint32_t o = 1; o < kJoinWaves * per; o++)
 #pragma unroll
                     for (int k = 0; k < kChunk; k++) acc[k] += sum[o / per][o % per * a.lanes + lane][k];
@@ -863,8 +875,8 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     hipError_t e = by_index(b.index_size, [&](auto iw) { return sort_records<decltype(iw)::value>(p, tab, b, w, err, s, &sorted); });
     if (e != hipSuccess) return e;
     const SumArgs a = {sorted, reinterpret_cast<float*>(w + p.first), reinterpret_cast<float*>(w + p.last), reinterpret_cast<uint32_t*>(w + p.joins),
-                       uint32_t(b.n), p.k, p.groups, p.pitch, p.lanes, divisor(p.chunks)};
-    const Divisor wide = divisor((tab.row_len + 64 * kChunk - 1) / (64 * kChunk));
+                       uint32_t(b.n), p.k, p.groups, p.pitch, std::min(p.lanes, tab.row_len > 1024 ? 32u : 16u), divisor(p.chunks)};
+    const Divisor wide = divisor((tab.row_len + a.lanes * kChunk - 1) / (a.lanes * kChunk));
     const unsigned join_blocks = unsigned(std::min<uint64_t>(uint64_t(p.groups) * wide.d, 512));
     const unsigned blocks = unsigned((uint64_t(p.groups) * p.chunks * p.lanes + 255) / 256);
     return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) {
