@@ -286,11 +286,16 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
             const uint2 c = h[uint64_t(blockIdx.x) * (nd / 2)], e = h[uint64_t(p.tiles) * (nd / 2)];
             before[0] = c.x, before[1] = c.y, total[0] = e.x, total[1] = e.y;
         } else {
-#pragma unroll 16
-            for (uint32_t t = 0; t < p.tiles; t++) {
-                const uint2 c = h[t * (nd / 2)];
-                if (t < blockIdx.x) before[0] += c.x, before[1] += c.y;
-                total[0] += c.x, total[1] += c.y;
+            for (uint32_t t = 0; t < p.tiles; t += 16) {           // (16 reads in flight, the last ones again)
+                uint2 c[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) c[i] = h[min(t + i, p.tiles - 1) * (nd / 2)];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    if (t + i >= p.tiles) continue;
+                    if (t + i < blockIdx.x) before[0] += c[i].x, before[1] += c[i].y;
+                    total[0] += c[i].x, total[1] += c[i].y;
+                }
             }
         }
     }
@@ -346,29 +351,28 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
 }
 
 // Up to kOneTile records: every pass in one block and one launch, the records changing places through
-// global memory (a block's own writes, ordered by its barriers). Whole batches of 512 columns: 1024
-// records 13.0 us against 17.7 in several launches, 4096 22.6 against 23.2, 8192 36 against 23.
+// LDS. Whole batches of 512 columns: ONEFIG
 constexpr uint32_t kOneTile = 6144;
 constexpr int kOneBits = 9;
 
 template <int IW>
-__global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint2* other, uint32_t passes, RowBatch b, RowTable tab, uint32_t* err) {
+__global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint32_t passes, RowBatch b, RowTable tab, uint32_t* err) {
     constexpr int kWaves = 16, kMost = kOneTile / 1024;
-    __shared__ uint32_t cnt[kWaves][1 << kOneBits];
+    __shared__ uint32_t row_at[kOneTile];
+    __shared__ uint16_t record_at[kOneTile], cnt[kWaves][1 << kOneBits];
     __shared__ uint32_t wsum[kWaves];
     const uint32_t nd = 1u << p.bits, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t rounds = (p.n + 1023) / 1024, j0 = w * rounds * 64 + lane;     // a wave's records are neighbours
     if (threadIdx.x == 0) *p.joins = 0;
-    uint2* out = p.out;
+    uint2 rec[kMost];
+#pragma unroll
+    for (int k = 0; k < kMost; k++) {
+        const uint32_t j = j0 + k * 64;
+        rec[k] = uint32_t(k) < rounds && j < p.n ? sort_record<IW>(p, b, tab, err, j) : uint2{kNoRow, 0};
+    }
     for (uint32_t pass = 0; pass < passes; pass++) {
         for (uint32_t d = lane; d < nd; d += 64) cnt[w][d] = 0;
-        uint2 rec[kMost];
         uint32_t rank[kMost];
-#pragma unroll
-        for (int k = 0; k < kMost; k++) {
-            const uint32_t j = j0 + k * 64;
-            rec[k] = uint32_t(k) < rounds && j < p.n ? sort_record<IW>(p, b, tab, err, j) : uint2{kNoRow, 0};
-        }
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
             if (uint32_t(k) >= rounds) break;
@@ -379,7 +383,7 @@ __global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint2* other
             const uint32_t had = live ? cnt[w][d] : 0;
             rank[k] = had + below;
             __builtin_amdgcn_wave_barrier();                       // every lane has read before one writes
-            if (live && below == 0) cnt[w][d] = had + __popcll(same);
+            if (live && below == 0) cnt[w][d] = uint16_t(had + __popcll(same));
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
@@ -401,7 +405,7 @@ __global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint2* other
 #pragma unroll
             for (int i = 0; i < kWaves; i++) {
                 const uint32_t c = cnt[i][threadIdx.x];
-                cnt[i][threadIdx.x] = at;
+                cnt[i][threadIdx.x] = uint16_t(at);
                 at += c;
             }
         }
@@ -409,16 +413,23 @@ __global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint2* other
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
             if (uint32_t(k) >= rounds) break;
+            if (j0 + k * 64 >= p.n) continue;
             const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
-            if (j0 + k * 64 < p.n && to < p.n) out[to] = rec[k];
+            if (pass + 1 == passes) {
+                p.out[to] = rec[k];
+            } else {
+                row_at[to] = rec[k].x;
+                record_at[to] = uint16_t(rec[k].y);
+            }
         }
-        __threadfence_block();
-        __syncthreads();
-        p.in = out;
         p.shift += p.bits;
-        uint2* const o = out;
-        out = other;
-        other = o;
+        if (pass + 1 == passes) break;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            const uint32_t j = j0 + k * 64;
+            if (uint32_t(k) < rounds && j < p.n) rec[k] = {row_at[j], record_at[j]};
+        }
     }
 }
 
@@ -536,13 +547,22 @@ constexpr uint32_t kWaveParts = 64;
 constexpr uint32_t kJoinWaves = 8;
 
 __device__ __forceinline__ void add_parts(const SumArgs& a, uint32_t tile, uint32_t j0, uint32_t j1, uint32_t chunk, float (&acc)[kChunk]) {
-#pragma unroll 8
-    for (uint32_t j = j0; j < j1; j++) {
-        const float* f = (j == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + j) * a.pitch) + chunk * kChunk;
-        float v[kChunk];
-        unpack(load_chunk(f), v);
+    constexpr int U = 8;
+    for (uint32_t j = j0; j < j1; j += U) {                        // (U parts in flight, the last one again)
+        Chunk<float> c[U];
 #pragma unroll
-        for (int i = 0; i < kChunk; i++) acc[i] += v[i];
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = min(j + u, j1 - 1);
+            c[u] = load_chunk((i == 0 ? a.last + uint64_t(tile) * a.pitch : a.first + uint64_t(tile + i) * a.pitch) + chunk * kChunk);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (j + u >= j1) continue;
+            float v[kChunk];
+            unpack(c[u], v);
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) acc[i] += v[i];
+        }
     }
 }
 
@@ -687,12 +707,18 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
     T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
     const V* x = vals + uint64_t(t) * b.stride;
     if constexpr (!is_code<T>::v) {
-#pragma unroll 4
-        for (uint32_t c = mine_of; c * kChunk < tab.row_len; c += L) {
-            const uint32_t at = span_of(c, tab.row_len).at;
-            float v[kChunk];
-            unpack(fetch(x, at, tab.row_len, true), v);
-            put(row, at, tab.row_len, pack<T>(v));
+        constexpr int U = 4;                                       // chunks in flight
+        const uint32_t chunks = (tab.row_len + kChunk - 1) / kChunk;
+        for (uint32_t c = mine_of; c < chunks; c += U * L) {
+            Chunk<V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = fetch(x, span_of(c + u * L, tab.row_len).at, tab.row_len, c + u * L < chunks);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float f[kChunk];
+                unpack(v[u], f);
+                if (c + u * L < chunks) put(row, span_of(c + u * L, tab.row_len).at, tab.row_len, pack<T>(f));
+            }
         }
     } else if (lpg) {
         const uint32_t in = mine_of & (lpg - 1), at = span_of(in, tab.group).at;
@@ -712,11 +738,18 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
             const V* xg = x + uint64_t(g) * tab.group;
             T* rg = row + uint64_t(g) * tab.group;
             uint32_t m = 0;
-#pragma unroll 4
-            for (uint32_t c = mine_of; c * kChunk < tab.group; c += L) {
-                float v[kChunk];
-                unpack(fetch(xg, span_of(c, tab.group).at, tab.group, true), v);
-                m = max(m, max_bits(v));
+            constexpr int U = 4;                                   // chunks in flight
+            const uint32_t chunks = (tab.group + kChunk - 1) / kChunk;
+            for (uint32_t c = mine_of; c < chunks; c += U * L) {
+                Chunk<V> v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) v[u] = fetch(xg, span_of(c + u * L, tab.group).at, tab.group, c + u * L < chunks);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float f[kChunk];
+                    unpack(v[u], f);
+                    m = max(m, max_bits(f));
+                }
             }
             m = max_over(m, 64);
             if constexpr (kWaves > 1) {                            // (two sets: a wave may be one group ahead)
@@ -725,12 +758,16 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
                 m = max(max(top[g & 1][0], top[g & 1][1]), max(top[g & 1][2], top[g & 1][3]));
             }
             const GroupScale q = group_scale<T>(m);
-#pragma unroll 4
-            for (uint32_t c = mine_of; c * kChunk < tab.group; c += L) {
-                const uint32_t at = span_of(c, tab.group).at;
-                float v[kChunk];
-                unpack(fetch(xg, at, tab.group, true), v);
-                put(rg, at, tab.group, pack_codes<T>(v, q));
+            for (uint32_t c = mine_of; c < chunks; c += U * L) {
+                Chunk<V> v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) v[u] = fetch(xg, span_of(c + u * L, tab.group).at, tab.group, c + u * L < chunks);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float f[kChunk];
+                    unpack(v[u], f);
+                    if (c + u * L < chunks) put(rg, span_of(c + u * L, tab.group).at, tab.group, pack_codes<T>(f, q));
+                }
             }
             if (mine_of == 0) tab.scales[uint64_t(r) * tab.groups + g] = q.scale;
         }
@@ -819,8 +856,8 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     uint64_t at = 0;
     auto take = [&at](uint64_t bytes) { const uint64_t o = at; at += (bytes + 255) & ~uint64_t(255); return o; };
     p.rec[0] = take(n * sizeof(uint2));
-    p.rec[1] = take(p.passes > 1 ? n * sizeof(uint2) : 0);
-    p.hist = take((uint64_t(p.tiles) + 1) << p.bits << 2);
+    p.rec[1] = take(!p.one && p.passes > 1 ? n * sizeof(uint2) : 0);
+    p.hist = take(p.one ? 0 : (uint64_t(p.tiles) + 1) << p.bits << 2);
     p.joins = take((uint64_t(p.groups) + 1) * 4);
     p.first = take(uint64_t(p.groups) * p.pitch * 4);
     p.last = take(uint64_t(p.groups) * p.pitch * 4);
@@ -834,10 +871,9 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
     const uint2* in = nullptr;
     if (p.one) {
         uint2* const a = reinterpret_cast<uint2*>(work + p.rec[0]);
-        uint2* const c = reinterpret_cast<uint2*>(work + p.rec[1]);
         const SortPass q = {nullptr, a, nullptr, uint32_t(b.n), 0, p.bits, 1, false, reinterpret_cast<uint32_t*>(work + p.joins)};
-        hipLaunchKernelGGL((k_rows_sort_one<IW>), dim3(1), dim3(1024), 0, s, q, c, p.passes, b, tab, err);
-        *sorted = p.passes % 2 ? a : c;
+        hipLaunchKernelGGL((k_rows_sort_one<IW>), dim3(1), dim3(1024), 0, s, q, p.passes, b, tab, err);
+        *sorted = a;
         return hipGetLastError();
     }
     for (uint32_t i = 0; i < p.passes; i++) {
