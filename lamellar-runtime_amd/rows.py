@@ -59,6 +59,7 @@ ROW_TYPES = {t.name: t for t in (
     RowType("f32", 0, torch.float32), RowType("f16", 1, torch.float16), RowType("bf16", 2, torch.bfloat16),
     RowType("i8", 3, torch.int8, 127.0), RowType("e4m3", 4, torch.float8_e4m3fn, 448.0))}
 _BY_TORCH = {t.torch: t for t in ROW_TYPES.values()}
+_VALUES = {k: t for t in ROW_TYPES.values() if not t.is_code for k in (t.name, t.torch)}
 MAX_ROW_LEN = 1 << 18                     # LMR_ROW_MAX_LEN
 MAX_ROWS = 0xFFFFFFF0                     # LMR_ROWS_MAX, of one PE
 SCAN = 1024                               # LMR_ROW_SCAN: stores of more records use claims
@@ -73,9 +74,9 @@ def row_type_of(t) -> RowType:
 
 
 def _value_type(t) -> RowType:
-    r = row_type_of(t)
-    if r.is_code:
-        raise LamellarError(LmrStatus.UNSUPPORTED, f"values are f32, f16 or bf16, not {r.name}")
+    r = _VALUES.get(t) if isinstance(t, (str, torch.dtype)) else row_type_of(t)
+    if r is None or r.is_code:
+        raise LamellarError(LmrStatus.UNSUPPORTED, f"values are f32, f16 or bf16, not {t}")
     return r
 
 
@@ -183,6 +184,8 @@ class RowArray:
         elif group is not None:
             raise LamellarError(LmrStatus.INVALID, f"{rt.name} rows have no groups")
         self.team, self.rtype, self.row_len, self.group = team, rt, row_len, group
+        self._out_type = ROW_TYPES["bf16"] if rt.is_code else rt
+        self._distributed = team.num_pes() > 1 or _FORCE_EXCHANGE
         self.layout = _capi.lmr_layout_t()
         check(_capi.lib().lmr_layout_new(ctypes.byref(self.layout), rows, team.num_pes(), team.my_pe(),
                                          int(distribution)), "lmr_layout_new")
@@ -242,7 +245,7 @@ class RowArray:
             if out_dtype is not None and _value_type(out_dtype) is not rt:
                 raise LamellarError(LmrStatus.INVALID, f"out is {rt.name}, not {out_dtype}")
         else:
-            rt = _value_type(out_dtype) if out_dtype is not None else ROW_TYPES["bf16"] if self.rtype.is_code else self.rtype
+            rt = self._out_type if out_dtype is None else _value_type(out_dtype)
         return RowsHandle(self, lambda: self._load(index, scale, rt, pad, out))
 
     def batch_add_rows(self, index, vals, scale=1.0, pad=None):
@@ -259,9 +262,6 @@ class RowArray:
         return RowsHandle(self, lambda: self._write(index, vals, 1.0, pad, False))
 
     # ---- one PE's part, and the exchange ----
-    def _distributed(self):
-        return self.team.num_pes() > 1 or _FORCE_EXCHANGE
-
     def _on_stream(self, k):
         """The current stream, which will use the array's memory: its reuse waits for that stream."""
         s = k.stream_id()
@@ -332,7 +332,7 @@ class RowArray:
         k = self.team.kernels
         idx, shape = self._index(k, index)
         n, shape = idx.numel(), (*shape, self.row_len)
-        alone = not self._distributed()
+        alone = not self._distributed
         stride = self.row_len
         if out is None:
             rows = out = torch.empty(shape, dtype=rt.torch, device=k.device)
@@ -372,7 +372,7 @@ class RowArray:
         n = idx.numel()
         vals, rt = self._values(k, vals, n)
         stream = self._on_stream(k)
-        if self._distributed():
+        if self._distributed:
             idx, vals, pad = self._exchange_values(k, idx, vals, pad)
             n = idx.numel()
         if n == 0:
