@@ -260,15 +260,22 @@ __global__ __launch_bounds__(64) void k_rows_prefix(SortPass p) {
     p.hist[uint64_t(p.tiles) * nd + d] = sum;
 }
 
-// the lanes of the wave whose digit is this lane's
-__device__ __forceinline__ uint64_t same_digit(uint32_t d, uint32_t bits, bool live) {
-    uint64_t same = __ballot(live);
-    for (uint32_t i = 0; i < bits; i++) {
-        const bool one = (d >> i) & 1;
-        const uint64_t m = __ballot(one);
-        same &= one ? m : ~m;
+// the lanes of the wave whose digit (below 2^MOST) is this lane's: a ballot per bit, kept where it agrees
+template <int MOST>
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, bool live) {
+    const uint64_t all = __ballot(live);
+    uint32_t lo = uint32_t(all), hi = uint32_t(all >> 32);
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+        const uint32_t one = uint32_t(int32_t(d << (31 - i)) >> 31);          // all ones or none
+        const uint64_t m = __ballot(one != 0);
+        lo &= ~(uint32_t(m) ^ one);
+        hi &= ~(uint32_t(m >> 32) ^ one);
     }
-    return same;
+    return uint64_t(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0));
 }
 
 template <int IW, int IPT>
@@ -324,8 +331,8 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     for (int k = 0; k < IPT; k++) {
         const bool live = j0 + k * 64 < p.n;
         const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
-        const uint64_t same = same_digit(d, p.bits, live);
-        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+        const uint64_t same = same_digit<kSortBits>(d, live);
+        const uint32_t below = lanes_below(same);
         const uint32_t had = live ? cnt[w][d] : 0;
         rank[k] = had + below;
         __builtin_amdgcn_wave_barrier();                           // every lane has read before one writes
@@ -376,11 +383,11 @@ __global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint32_t pas
         uint32_t rank[kMost];
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
-            if (uint32_t(k) >= rounds) break;
+            if (uint32_t(k) >= rounds) continue;
             const bool live = j0 + k * 64 < p.n;
             const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
-            const uint64_t same = same_digit(d, p.bits, live);
-            const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+            const uint64_t same = same_digit<kOneBits>(d, live);
+            const uint32_t below = lanes_below(same);
             const uint32_t had = live ? cnt[w][d] : 0;
             rank[k] = had + below;
             __builtin_amdgcn_wave_barrier();                       // every lane has read before one writes
@@ -413,8 +420,7 @@ __global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint32_t pas
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
-            if (uint32_t(k) >= rounds) break;
-            if (j0 + k * 64 >= p.n) continue;
+            if (uint32_t(k) >= rounds || j0 + k * 64 >= p.n) continue;
             const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
             if (pass + 1 == passes) {
                 p.out[to] = rec[k];
