@@ -18,6 +18,9 @@
  *           495-530).                                  -> lmr_scatter_results
  *   reductions (unsafe.rs:1414-1557, array_reduce.rs)    -> lmr_reduce
  *
+ * Beside it, batches whose record is a whole row of a table (no counterpart in the
+ * reference): lmr_rows_load / lmr_rows_add / lmr_rows_store.
+ *
  * Conventions
  *  - Pointers named d_* are device (HBM) pointers; everything else is host.
  *  - Every device call is stream-ordered and asynchronous; `stream` is a
@@ -502,7 +505,7 @@ lmr_status_t lmr_reduce(lmr_ctx_t* ctx, uint32_t dtype, uint32_t op, const void*
  *               They must not overlap the table.
  * Arithmetic is f32, rounded once (to nearest, ties to even) where a narrower type is written.
  * Nothing is allocated and nothing waits; every call may be captured into a graph. They use none of
- * the context's workspace (only its device and error word): calls on different tables may run on
+ * the context's workspace (only its device and error word; no stage timing): calls on different tables may run on
  * several streams at once, calls that write one table must be ordered by the caller. n <= LMR_ROW_MAX_BATCH, n * row_len <= LMR_ROW_MAX_VALUES,
  * stride <= LMR_ROW_MAX_STRIDE. */
 #define LMR_ROW_MAX_LEN (1u << 18)

@@ -124,16 +124,14 @@ __device__ __forceinline__ void add_to_row(T* row, const Span& sp, Chunk<T> old,
 }
 
 // ---------------------------------------------------------------- add, few records
-// One launch: a block per record and 512 columns. Each wave finds the record's row in the whole list
-// (kFewRecords indices, 8 a lane); a record with an earlier one of its row leaves. The first sums the
-// row's records in order, its four waves a quarter each where there are more than four. 512 records of
-// 1024: 4.9 us, sorted 12.4. The work grows with the square of the batch: 768 records of 4096 take 29 us
-// this way and 15 sorted.
-constexpr int kFewRecords = 512;
-
-template <typename T, typename V, int IW>
+// One launch: a block per record and 512 columns. Each wave finds the record's row in the whole list (MOST
+// indices at most); a record with an earlier one of its row leaves. The first sums the row's records in
+// order, its four waves a quarter each where there are more than four. The blocks' number and their work
+// both grow with the batch (add_plan says how far): 512 records of 1024 4.9 us, 10.7 sorted; 1024 of 1024
+// 9.0 and 11.9; 512 of 8192 18.2 and 14.8; 1024 of 2048 15.7 and 12.6.
+template <typename T, typename V, int IW, int MOST>
 __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, const V* vals, uint32_t* err) {
-    __shared__ uint16_t list[kFewRecords];
+    __shared__ uint16_t list[MOST];
     __shared__ float sum[3][64][kChunk + 1];
     const uint32_t t = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t r = row_of<IW>(b, t, tab.rows, err, threadIdx.x == 0 && blockIdx.y == 0);
@@ -143,16 +141,16 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
     T* row = reinterpret_cast<T*>(tab.data) + uint64_t(r) * tab.row_len;
     const Chunk<T> old = fetch(row, sp.at, tab.row_len, on && w == 0);
     uint32_t total = 0;
-    bool hit[kFewRecords / 64], earlier = false;
+    bool hit[MOST / 64], earlier = false;
 #pragma unroll
-    for (int i = 0; i < kFewRecords / 64; i++) {
+    for (int i = 0; i < MOST / 64; i++) {
         const uint32_t u = i * 64 + lane;
         hit[i] = u < b.n && row_index<IW>(b, u) == r;
         earlier |= hit[i] && u < t;
     }
     if (__ballot(earlier)) return;                                 // (alike in every wave)
 #pragma unroll
-    for (int i = 0; i < kFewRecords / 64; i++) {
+    for (int i = 0; i < MOST / 64; i++) {
         const uint64_t m = __ballot(hit[i]);
         if (hit[i] && w == 0) list[total + __popcll(m & ((1ull << lane) - 1))] = uint16_t(i * 64 + lane);
         total += __popcll(m);
@@ -200,8 +198,8 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
 // counts the digits of its tile, then places its tile behind what earlier tiles and lower digits
 // take. Records keep their order among equal digits: a wave ranks its 64 records by ballots, waves
 // and tiles follow one another in order. Bound by the latency of its launches (a pass over 16384 records
-// 6.9 us, over 131072 13 us), so tiles are small while they are few: 16384 records in tiles of 2048 took
-// 7 us longer than in tiles of 512.
+// 6.6 us, over 131072 14 us), so tiles are small while they are few (whole batches of 512 columns: 8192
+// records 22.5, 24.0, 27.2 us in tiles of 512, 1024, 2048, 65536 66.6, 60.5, 61.0, 131072 87, 84, 79).
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kSortBits = 10;
@@ -832,7 +830,8 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
 // How a batch of adds runs, and its workspace: two lists of (row, record), the digit counts, and the
 // parts of rows that reach past a group's records.
 struct AddPlan {
-    bool few, one;
+    uint32_t few;                            // k_rows_add_few for at most so many records, 0: sorted
+    bool one;
     uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
     uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
     uint32_t pitch;
@@ -840,22 +839,23 @@ struct AddPlan {
 };
 AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     AddPlan p = {};
-    p.few = n <= kFewRecords;
+    const uint64_t blocks = n * ((row_len + 511) / 512);
+    p.few = n <= 512 && blocks <= 4096 ? 512 : n <= 1024 && blocks <= 2560 ? 1024 : 0;
     if (p.few) return p;
     const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
     p.one = n <= kOneTile;
     const uint32_t most = p.one ? kOneBits : kSortBits;
     p.passes = (key_bits + most - 1) / most;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    // (tiles of 512, 1024, 2048 and 8192 records: at most 128 of them up to 2^18 records)
+    // (tiles of 512, 1024, 2048 and 8192 records: see k_rows_place; at most 128 of them up to 2^18 records)
     p.ipt = n <= 16384 ? 1 : n <= 65536 ? 2 : n <= 262144 ? 4 : 16;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
     p.chunks = (cols + p.lanes - 1) / p.lanes;
     // 32 records a group, fewer where that would leave less than about 8 waves per compute unit (131072
-    // records of 4096, all launches: 564, 519, 510, 505 us with 8, 16, 24, 32; 5003 of 1001: 34.4, 36.9, 43
-    // us with 4, 8, 16)
+    // records of 4096, all launches: 647, 557, 516, 504 us with 4, 8, 16, 32; 5003 of 1001: 28.9, 32.0, 38.9
+    // with 4, 8, 16)
     const uint64_t waves = n * p.chunks * p.lanes / 64;
     p.k = waves >= 32 * 2048 ? 32 : waves >= 16 * 2048 ? 16 : waves >= 8 * 2048 ? 8 : 4;
     p.groups = uint32_t((n + p.k - 1) / p.k);
@@ -908,9 +908,11 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
     const AddPlan p = add_plan(tab.rows, tab.row_len, b.n);
     if (p.few)
         return by_value_type(tab.type, [&](auto t) { return by_value_type(val_type, [&](auto v) { return by_index(b.index_size, [&](auto iw) {
-            hipLaunchKernelGGL((k_rows_add_few<decltype(t), decltype(v), decltype(iw)::value>),
-                               dim3(unsigned(b.n), (tab.row_len + 511) / 512), dim3(256), 0, s, tab, b,
-                               reinterpret_cast<const decltype(v)*>(vals), err);
+            using V = decltype(v);
+            const dim3 grid(unsigned(b.n), (tab.row_len + 511) / 512);
+            const V* x = reinterpret_cast<const V*>(vals);
+            if (p.few == 512) hipLaunchKernelGGL((k_rows_add_few<decltype(t), V, decltype(iw)::value, 512>), grid, dim3(256), 0, s, tab, b, x, err);
+            else hipLaunchKernelGGL((k_rows_add_few<decltype(t), V, decltype(iw)::value, 1024>), grid, dim3(256), 0, s, tab, b, x, err);
             return hipGetLastError();
         }); }); });
     uint8_t* w = reinterpret_cast<uint8_t*>(work);
@@ -938,7 +940,8 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
             default: sum(std::integral_constant<int, 64>{}, whole, u);
             }
         };
-        // (131072 bf16 records of 4096: 512 us with 4 in flight, 502 with 8; 5003 of 1001: 36.8 and 38.4)
+        // (131072 bf16 records of 4096: 514 us with 4 in flight, 504 with 8; ends of rows that are not whole cost
+        // registers: 5003 of 1001 took 1.5 us longer with 8)
         if (tab.row_len % kChunk) by_lanes(std::false_type{}, std::integral_constant<int, 4>{});
         else if (p.k == 4) by_lanes(std::true_type{}, std::integral_constant<int, 4>{});
         else by_lanes(std::true_type{}, std::integral_constant<int, 8>{});

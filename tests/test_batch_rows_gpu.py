@@ -165,7 +165,8 @@ def test_load_shapes_strides_and_inputs(lam, world):
                                        ("f32", "f16")])
 @pytest.mark.parametrize("n,rows,width,how", [
     (1, 1, 1, "same"), (2, 1, 3, "same"), (5, 9, 64, "any"), (63, 700, 1001, "distinct"), (300, 7, 520, "any"),
-    (511, 600, 33, "skewed"), (512, 600, 8, "any"), (513, 600, 40, "skewed"), (1025, 70, 1024, "skewed"), (1500, 1, 72, "same"),
+    (511, 600, 33, "skewed"), (512, 600, 8, "any"), (513, 600, 40, "skewed"), (1024, 900, 1024, "skewed"), (1025, 70, 1024, "skewed"),
+    (700, 9, 1500, "few"), (513, 400, 2600, "skewed"), (257, 100, 8200, "skewed"), (1500, 1, 72, "same"),
     (4096, 5000, 130, "few"), (4099, 4099, 264, "distinct"), (9000, 100000, 96, "any"), (20000, 1 << 19, 24, "skewed")])
 def test_add(lam, world, kind, vals, n, rows, width, how):
     g = gen(n + width)
