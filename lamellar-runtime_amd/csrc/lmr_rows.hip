@@ -199,7 +199,10 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
 // take. Records keep their order among equal digits: a wave ranks its 64 records by ballots, waves
 // and tiles follow one another in order. Bound by the latency of its launches (a pass over 16384 records
 // 6.6 us, over 131072 14 us), so tiles are small while they are few (whole batches of 512 columns: 8192
-// records 22.5, 24.0, 27.2 us in tiles of 512, 1024, 2048, 65536 66.6, 60.5, 61.0, 131072 87, 84, 79).
+// records 22.5, 24.0, 27.2 us in tiles of 512, 1024, 2048; of 16 columns in tiles of 1024, 2048, 4096, 8192:
+// 262144 records 43.9, 46.5, 51.9, 63.6 us, 600000 71.0, 69.0, 69.4, 83.5, 2 million 239, 219, 211, 218,
+// 8 million 815, 736, 695, 696). With more than 64 tiles a launch of its own adds up their counts: 65536
+// records of 64 columns 34.6 us with it, 33.9 without, 300000 51 us with it, 74 in tiles large enough to do without.
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kSortBits = 10;
@@ -238,24 +241,39 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_count(SortPass p, RowBatc
     for (uint32_t d = threadIdx.x; d < nd; d += kSortThreads) p.hist[uint64_t(blockIdx.x) * nd + d] = cnt[d];
 }
 
-// many tiles: each digit's counts become the counts of the tiles before, the totals go behind them
-__global__ __launch_bounds__(64) void k_rows_prefix(SortPass p) {
-    const uint32_t nd = 1u << p.bits, d = blockIdx.x * 64 + threadIdx.x;
+// many tiles: each digit's counts become the counts of the tiles before, the totals go behind them. A block
+// has 64 digits, its 16 waves a sixteenth of the tiles each: their sums first, then the counts again
+__global__ __launch_bounds__(1024) void k_rows_prefix(SortPass p) {
+    __shared__ uint32_t part[16][64];
+    const uint32_t nd = 1u << p.bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+    const uint32_t share = (p.tiles + 15) / 16, t0 = min(p.tiles, w * share), t1 = min(p.tiles, t0 + share);
+    constexpr int U = 16;                                          // reads in flight
+    uint32_t sum = 0;
+    if (d < nd)
+        for (uint32_t t = t0; t < t1; t += U) {
+            uint32_t c[U];
+#pragma unroll
+            for (int i = 0; i < U; i++) c[i] = p.hist[uint64_t(min(t + i, t1 - 1)) * nd + d];
+#pragma unroll
+            for (int i = 0; i < U; i++) sum += t + i < t1 ? c[i] : 0;
+        }
+    part[w][lane] = sum;
+    __syncthreads();
+    sum = 0;
+    for (uint32_t i = 0; i < w; i++) sum += part[i][lane];
     if (d >= nd) return;
-    uint32_t sum = 0, t = 0;
-    for (; t + 16 <= p.tiles; t += 16) {
-        uint32_t c[16];
+    for (uint32_t t = t0; t < t1; t += U) {
+        uint32_t c[U];
 #pragma unroll
-        for (int i = 0; i < 16; i++) c[i] = p.hist[uint64_t(t + i) * nd + d];
+        for (int i = 0; i < U; i++) c[i] = p.hist[uint64_t(min(t + i, t1 - 1)) * nd + d];
 #pragma unroll
-        for (int i = 0; i < 16; i++) { p.hist[uint64_t(t + i) * nd + d] = sum; sum += c[i]; }
+        for (int i = 0; i < U; i++) {
+            if (t + i >= t1) continue;
+            p.hist[uint64_t(t + i) * nd + d] = sum;
+            sum += c[i];
+        }
     }
-    for (; t < p.tiles; t++) {
-        const uint32_t c = p.hist[uint64_t(t) * nd + d];
-        p.hist[uint64_t(t) * nd + d] = sum;
-        sum += c;
-    }
-    p.hist[uint64_t(p.tiles) * nd + d] = sum;
+    if (w == 15) p.hist[uint64_t(p.tiles) * nd + d] = sum;
 }
 
 // the lanes of the wave whose digit (below 2^MOST) is this lane's: a ballot per bit, kept where it agrees
@@ -847,8 +865,8 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     const uint32_t most = p.one ? kOneBits : kSortBits;
     p.passes = (key_bits + most - 1) / most;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    // (tiles of 512, 1024, 2048 and 8192 records: see k_rows_place; at most 128 of them up to 2^18 records)
-    p.ipt = n <= 16384 ? 1 : n <= 65536 ? 2 : n <= 262144 ? 4 : 16;
+    // (tiles of 512, 1024, 2048 and 4096 records: see above kSortThreads)
+    p.ipt = n <= 16384 ? 1 : n <= (1 << 18) ? 2 : n <= (1 << 20) ? 4 : 8;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
@@ -885,18 +903,18 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
     }
     for (uint32_t i = 0; i < p.passes; i++) {
         uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
-        SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 128,
+        SortPass q = {in, out, reinterpret_cast<uint32_t*>(work + p.hist), uint32_t(b.n), i * p.bits, p.bits, p.tiles, p.tiles > 64,
                       reinterpret_cast<uint32_t*>(work + p.joins)};
         auto go = [&](auto ipt) {
             constexpr int IPT = decltype(ipt)::value;
             hipLaunchKernelGGL((k_rows_count<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
-            if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(64), 0, s, q);
+            if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(1024), 0, s, q);
             hipLaunchKernelGGL((k_rows_place<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
         };
         if (p.ipt == 1) go(std::integral_constant<int, 1>{});
         else if (p.ipt == 2) go(std::integral_constant<int, 2>{});
         else if (p.ipt == 4) go(std::integral_constant<int, 4>{});
-        else go(std::integral_constant<int, 16>{});
+        else go(std::integral_constant<int, 8>{});
         in = out;
     }
     *sorted = in;

@@ -191,6 +191,22 @@ def test_add_large(lam, world, n, rows, width, how):
     check_close(a.local_rows(), exact, bound)
 
 
+@pytest.mark.parametrize("n", [16384, 16385, 65536, 65537, 262143, 262145, 1 << 20, (1 << 20) + 1, 3000001])
+@pytest.mark.parametrize("rows", [700, 3000017])
+def test_add_many_records(lam, world, n, rows):
+    """Sort tiles of each size, few and many of them. Whole numbers: the sums are exact (below 2^24: a row
+    has at most 16 n / rows + 2^16 records of at most 8)."""
+    g = gen(n)
+    a = lam.RowArray(world.team(), rows, 2)
+    i = torch.where(torch.rand(n, generator=g) < 0.5, torch.randint(rows, (n,), generator=g),
+                    torch.randint(rows // 16 + 1, (n,), generator=g))
+    i[-1], i[0] = rows - 1, 0
+    v = torch.randint(-8, 9, (n, 2), generator=g)
+    a.batch_add_rows(i.cuda(), v.float().cuda()).block()
+    exp = torch.zeros(rows, 2, dtype=torch.float64).index_add_(0, i, v.double())
+    assert torch.equal(a.local_rows().double().cpu(), exp)
+
+
 @pytest.mark.parametrize("n", [700, 6144, 6145, 20000])
 @pytest.mark.parametrize("rows", [3, 511, 512, (1 << 18) - 1, 1 << 18, (1 << 20) + 7, (1 << 27) + 3])
 def test_add_key_widths(lam, world, n, rows):
