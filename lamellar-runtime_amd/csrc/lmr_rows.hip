@@ -127,8 +127,8 @@ __device__ __forceinline__ void add_to_row(T* row, const Span& sp, Chunk<T> old,
 // One launch: a block per record and 512 columns. Each wave finds the record's row in the whole list (MOST
 // indices at most); a record with an earlier one of its row leaves. The first sums the row's records in
 // order, its four waves a quarter each where there are more than four. The blocks' number and their work
-// both grow with the batch (add_plan says how far): 512 records of 1024 4.9 us, 10.7 sorted; 1024 of 1024
-// 9.0 and 11.9; 512 of 8192 18.2 and 14.8; 1024 of 2048 15.7 and 12.6.
+// both grow with the batch (add_plan says how far): 512 records of 1024 4.9 us, 8.6 sorted; 1024 of 1024
+// 8.9 and 9.7; 512 of 4096 10.2 and 9.9; 600 of 2048 10.1 and 9.3, 1024 15.4 and 10.2.
 template <typename T, typename V, int IW, int MOST>
 __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, const V* vals, uint32_t* err) {
     __shared__ uint16_t list[MOST];
@@ -276,13 +276,12 @@ __global__ __launch_bounds__(1024) void k_rows_prefix(SortPass p) {
     if (w == 15) p.hist[uint64_t(p.tiles) * nd + d] = sum;
 }
 
-// the lanes of the wave whose digit (below 2^MOST) is this lane's: a ballot per bit, kept where it agrees
-template <int MOST>
+// the lanes of the wave whose digit is this lane's: a ballot per bit, kept where it agrees
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool live) {
     const uint64_t all = __ballot(live);
     uint32_t lo = uint32_t(all), hi = uint32_t(all >> 32);
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
+    for (int i = 0; i < kSortBits; i++) {
         const uint32_t one = uint32_t(int32_t(d << (31 - i)) >> 31);          // all ones or none
         const uint64_t m = __ballot(one != 0);
         lo &= ~(uint32_t(m) ^ one);
@@ -347,7 +346,7 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     for (int k = 0; k < IPT; k++) {
         const bool live = j0 + k * 64 < p.n;
         const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
-        const uint64_t same = same_digit<kSortBits>(d, live);
+        const uint64_t same = same_digit(d, live);
         const uint32_t below = lanes_below(same);
         const uint32_t had = live ? cnt[w][d] : 0;
         rank[k] = had + below;
@@ -373,86 +372,67 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
     }
 }
 
-// Up to kOneTile records: every pass in one block and one launch, the records changing places through
-// LDS. Whole batches of 512 columns: 1024 records 12 us against 17 in several launches, 4096 19 against 19,
-// 6144 24.5 against 21.4.
-constexpr uint32_t kOneTile = 5120;
-constexpr int kOneBits = 9;
+// Up to kRankMost records: one launch, in which each block counts, for the records of its own, how many of
+// the whole list come before them: rows below theirs, and equal rows of earlier records. The list stands in
+// LDS; a thread compares four of its rows at a time with R records' (a record's count from `shares` threads).
+// Bound by n^2 comparisons of two instructions, 64 at a time, spread over all compute units: a block has a
+// 256th of the records, at least 16. Sums of 64 columns: 1500 records 10.4 us, 13.4 with a sort by digits in
+// one block, 5003 13.3 and 19.9, 8192 17.1 and 20.1 with tiles of many blocks; 10000 would take 27 and 21.6.
+// (5003 in blocks of 32: 14.4; 8192 in blocks of 16 19.3, of 64 22.7, with one record a thread 18.5.)
+constexpr uint32_t kRankMost = 8192;
 
 template <int IW>
-__global__ __launch_bounds__(1024) void k_rows_sort_one(SortPass p, uint32_t passes, RowBatch b, RowTable tab, uint32_t* err) {
-    constexpr int kWaves = 16, kMost = kOneTile / 1024;
-    __shared__ uint32_t row_at[kOneTile];
-    __shared__ uint16_t record_at[kOneTile], cnt[kWaves][1 << kOneBits];
-    __shared__ uint32_t wsum[kWaves];
-    const uint32_t nd = 1u << p.bits, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t rounds = (p.n + 1023) / 1024, j0 = w * rounds * 64 + lane;     // a wave's records are neighbours
-    if (threadIdx.x == 0) *p.joins = 0;
-    uint2 rec[kMost];
+__global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, RowBatch b, RowTable tab, uint32_t* err) {
+    constexpr int R = 2, U = 4;                                    // a thread's records, its reads in flight
+    __shared__ uint4 rows_at[kRankMost / 4];
+    __shared__ uint32_t rank[32];
+    const uint32_t padded = (p.n + 3) & ~3u, first = blockIdx.x * part, wide = part / R;
+    const uint32_t mine = threadIdx.x % wide * R, share = threadIdx.x / wide, shares = 1024 / wide;
+    uint32_t* const row_at = reinterpret_cast<uint32_t*>(rows_at);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.joins = 0;
+    if (threadIdx.x < part) rank[threadIdx.x] = 0;
+    for (uint32_t j0 = threadIdx.x; j0 < padded; j0 += 1024 * U) {
+        uint32_t row[U];
 #pragma unroll
-    for (int k = 0; k < kMost; k++) {
-        const uint32_t j = j0 + k * 64;
-        rec[k] = uint32_t(k) < rounds && j < p.n ? sort_record<IW>(p, b, tab, err, j) : uint2{kNoRow, 0};
+        for (int u = 0; u < U; u++) {
+            const uint32_t j = j0 + u * 1024;
+            const int64_t r = j < p.n ? row_of<IW>(b, j, tab.rows, err, j - first < part) : 0;
+            row[u] = j >= p.n ? kNoRow : r < 0 ? uint32_t(tab.rows) : uint32_t(r);     // (kNoRow is below none)
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (j0 + u * 1024 < padded) row_at[j0 + u * 1024] = row[u];
     }
-    for (uint32_t pass = 0; pass < passes; pass++) {
-        for (uint32_t d = lane; d < nd; d += 64) cnt[w][d] = 0;
-        uint32_t rank[kMost];
+    __syncthreads();
+    uint32_t row[R], before[R];
 #pragma unroll
-        for (int k = 0; k < kMost; k++) {
-            if (uint32_t(k) >= rounds) continue;
-            const bool live = j0 + k * 64 < p.n;
-            const uint32_t d = (rec[k].x >> p.shift) & (nd - 1);
-            const uint64_t same = same_digit<kOneBits>(d, live);
-            const uint32_t below = lanes_below(same);
-            const uint32_t had = live ? cnt[w][d] : 0;
-            rank[k] = had + below;
-            __builtin_amdgcn_wave_barrier();                       // every lane has read before one writes
-            if (live && below == 0) cnt[w][d] = uint16_t(had + __popcll(same));
-            __builtin_amdgcn_wave_barrier();
+    for (int k = 0; k < R; k++) {
+        const uint32_t i = first + mine + k;
+        row[k] = i < p.n ? row_at[i] : 0;
+        before[k] = 0;
+    }
+#pragma unroll 4
+    for (uint32_t c = share < shares ? share : padded; c < padded / 4; c += shares) {
+        const uint4 r = rows_at[c];
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const uint32_t limit = row[k] + (c * 4 < first + mine + k);                // equal rows count too
+            before[k] += (r.x < limit) + (r.y < limit) + (r.z < limit) + (r.w < limit);
         }
-        __syncthreads();
-        uint32_t total = 0;
-        if (threadIdx.x < nd)
+    }
 #pragma unroll
-            for (int i = 0; i < kWaves; i++) total += cnt[i][threadIdx.x];
-        uint32_t run = total;
+    for (int k = 0; k < R; k++) {
+        const uint32_t i = first + mine + k;
+        if (share == 0 && i < p.n && i % 4)                        // but for the record itself and its four's later ones
+            for (uint32_t j = i; j <= (i | 3); j++) before[k] -= row_at[j] == row[k];
+        atomicAdd(&rank[mine + k], before[k]);
+    }
+    __syncthreads();
+    if (share != 0) return;
 #pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t o = __shfl_up(run, s, 64);
-            if (int(lane) >= s) run += o;
-        }
-        if (lane == 63) wsum[w] = run;
-        __syncthreads();
-        if (threadIdx.x < nd) {
-            uint32_t at = run - total;
-            for (uint32_t i = 0; i < w; i++) at += wsum[i];
-#pragma unroll
-            for (int i = 0; i < kWaves; i++) {
-                const uint32_t c = cnt[i][threadIdx.x];
-                cnt[i][threadIdx.x] = uint16_t(at);
-                at += c;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kMost; k++) {
-            if (uint32_t(k) >= rounds || j0 + k * 64 >= p.n) continue;
-            const uint32_t to = cnt[w][(rec[k].x >> p.shift) & (nd - 1)] + rank[k];
-            if (pass + 1 == passes) {
-                p.out[to] = rec[k];
-            } else {
-                row_at[to] = rec[k].x;
-                record_at[to] = uint16_t(rec[k].y);
-            }
-        }
-        p.shift += p.bits;
-        if (pass + 1 == passes) break;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kMost; k++) {
-            const uint32_t j = j0 + k * 64;
-            if (uint32_t(k) < rounds && j < p.n) rec[k] = {row_at[j], record_at[j]};
-        }
+    for (int k = 0; k < R; k++) {
+        const uint32_t i = first + mine + k;
+        if (i < p.n) p.out[rank[mine + k]] = {row[k], i};
     }
 }
 
@@ -849,7 +829,7 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
 // parts of rows that reach past a group's records.
 struct AddPlan {
     uint32_t few;                            // k_rows_add_few for at most so many records, 0: sorted
-    bool one;
+    bool ranked;                             // k_rows_rank, not a sort by digits
     uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
     uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
     uint32_t pitch;
@@ -858,12 +838,11 @@ struct AddPlan {
 AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     AddPlan p = {};
     const uint64_t blocks = n * ((row_len + 511) / 512);
-    p.few = n <= 512 && blocks <= 4096 ? 512 : n <= 1024 && blocks <= 2560 ? 1024 : 0;
+    p.few = n <= 512 && blocks <= 4096 ? 512 : n <= 1024 && blocks <= 2048 ? 1024 : 0;
     if (p.few) return p;
     const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
-    p.one = n <= kOneTile;
-    const uint32_t most = p.one ? kOneBits : kSortBits;
-    p.passes = (key_bits + most - 1) / most;
+    p.ranked = n <= kRankMost;
+    p.passes = (key_bits + kSortBits - 1) / kSortBits;
     p.bits = (key_bits + p.passes - 1) / p.passes;
     // (tiles of 512, 1024, 2048 and 4096 records: see above kSortThreads)
     p.ipt = n <= 16384 ? 1 : n <= (1 << 18) ? 2 : n <= (1 << 20) ? 4 : 8;
@@ -881,8 +860,8 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     uint64_t at = 0;
     auto take = [&at](uint64_t bytes) { const uint64_t o = at; at += (bytes + 255) & ~uint64_t(255); return o; };
     p.rec[0] = take(n * sizeof(uint2));
-    p.rec[1] = take(!p.one && p.passes > 1 ? n * sizeof(uint2) : 0);
-    p.hist = take(p.one ? 0 : (uint64_t(p.tiles) + 1) << p.bits << 2);
+    p.rec[1] = take(!p.ranked && p.passes > 1 ? n * sizeof(uint2) : 0);
+    p.hist = take(p.ranked ? 0 : (uint64_t(p.tiles) + 1) << p.bits << 2);
     p.joins = take((uint64_t(p.groups) + 1) * 4);
     p.first = take(uint64_t(p.groups) * p.pitch * 4);
     p.last = take(uint64_t(p.groups) * p.pitch * 4);
@@ -894,10 +873,11 @@ template <int IW>
 hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b, uint8_t* work, uint32_t* err, hipStream_t s,
                         const uint2** sorted) {
     const uint2* in = nullptr;
-    if (p.one) {
+    if (p.ranked) {
         uint2* const a = reinterpret_cast<uint2*>(work + p.rec[0]);
-        const SortPass q = {nullptr, a, nullptr, uint32_t(b.n), 0, p.bits, 1, false, reinterpret_cast<uint32_t*>(work + p.joins)};
-        hipLaunchKernelGGL((k_rows_sort_one<IW>), dim3(1), dim3(1024), 0, s, q, p.passes, b, tab, err);
+        const SortPass q = {nullptr, a, nullptr, uint32_t(b.n), 0, 0, 1, false, reinterpret_cast<uint32_t*>(work + p.joins)};
+        const uint32_t part = std::max<uint32_t>(16, uint32_t(b.n + 511) / 512 * 2);       // 256 blocks
+        hipLaunchKernelGGL((k_rows_rank<IW>), dim3((uint32_t(b.n) + part - 1) / part), dim3(1024), 0, s, q, part, b, tab, err);
         *sorted = a;
         return hipGetLastError();
     }
