@@ -194,12 +194,11 @@ __global__ __launch_bounds__(256) void k_rows_add_few(RowTable tab, RowBatch b, 
 // ---------------------------------------------------------------- add, many records
 // The records sorted by row (and by place inside a row), then summed run by run.
 //
-// Sort: least significant digit first, digits of up to 10 bits. A pass is two launches: each block
+// Sort of many: least significant digit first, digits of up to 10 bits. A pass is two launches: each block
 // counts the digits of its tile, then places its tile behind what earlier tiles and lower digits
 // take. Records keep their order among equal digits: a wave ranks its 64 records by ballots, waves
-// and tiles follow one another in order. Bound by the latency of its launches (a pass over 16384 records
-// 6.6 us, over 131072 14 us), so tiles are small while they are few (whole batches of 512 columns: 8192
-// records 22.5, 24.0, 27.2 us in tiles of 512, 1024, 2048; of 16 columns in tiles of 1024, 2048, 4096, 8192:
+// and tiles follow one another in order. Bound by the latency of its launches (a pass over 131072 records
+// 14 us), so tiles are small while they are few (whole batches of 16 columns in tiles of 1024, 2048, 4096, 8192:
 // 262144 records 43.9, 46.5, 51.9, 63.6 us, 600000 71.0, 69.0, 69.4, 83.5, 2 million 239, 219, 211, 218,
 // 8 million 815, 736, 695, 696). With more than 64 tiles a launch of its own adds up their counts: 65536
 // records of 64 columns 34.6 us with it, 33.9 without, 300000 51 us with it, 74 in tiles large enough to do without.
@@ -377,16 +376,18 @@ __global__ __launch_bounds__(kSortThreads) void k_rows_place(SortPass p, RowBatc
 // LDS; a thread compares four of its rows at a time with R records' (a record's count from `shares` threads).
 // Bound by n^2 comparisons of two instructions, 64 at a time, spread over all compute units: a block has a
 // 256th of the records, at least 16. Sums of 64 columns: 1500 records 10.4 us, 13.4 with a sort by digits in
-// one block, 5003 13.3 and 19.9, 8192 17.1 and 20.1 with tiles of many blocks; 10000 would take 27 and 21.6.
-// (5003 in blocks of 32: 14.4; 8192 in blocks of 16 19.3, of 64 22.7, with one record a thread 18.5.)
-constexpr uint32_t kRankMost = 8192;
+// one block, 5003 13.3 and 19.9, 8192 17.1 and 15.1 with k_rows_merge (5003 in blocks of 32: 14.4; 8192 in
+// blocks of 16 19.3, of 64 22.7, with one record a thread 18.5).
+constexpr uint32_t kRankMost = 6144;
 
-template <int IW>
+// (TILE: the records of the block's tile of the list, not the whole list)
+template <int IW, uint32_t TILE>
 __global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, RowBatch b, RowTable tab, uint32_t* err) {
     constexpr int R = 2, U = 4;                                    // a thread's records, its reads in flight
-    __shared__ uint4 rows_at[kRankMost / 4];
-    __shared__ uint32_t rank[32];
-    const uint32_t padded = (p.n + 3) & ~3u, first = blockIdx.x * part, wide = part / R;
+    __shared__ uint4 rows_at[TILE / 4];
+    __shared__ uint32_t rank[64];
+    const uint32_t base = blockIdx.x * part / TILE * TILE, count = min(TILE, p.n - base), padded = (count + 3) & ~3u;
+    const uint32_t first = blockIdx.x * part - base, wide = part / R;
     const uint32_t mine = threadIdx.x % wide * R, share = threadIdx.x / wide, shares = 1024 / wide;
     uint32_t* const row_at = reinterpret_cast<uint32_t*>(rows_at);
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.joins = 0;
@@ -396,8 +397,8 @@ __global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, R
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t j = j0 + u * 1024;
-            const int64_t r = j < p.n ? row_of<IW>(b, j, tab.rows, err, j - first < part) : 0;
-            row[u] = j >= p.n ? kNoRow : r < 0 ? uint32_t(tab.rows) : uint32_t(r);     // (kNoRow is below none)
+            const int64_t r = j < count ? row_of<IW>(b, base + j, tab.rows, err, j - first < part) : 0;
+            row[u] = j >= count ? kNoRow : r < 0 ? uint32_t(tab.rows) : uint32_t(r);     // (kNoRow is below none)
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, R
 #pragma unroll
     for (int k = 0; k < R; k++) {
         const uint32_t i = first + mine + k;
-        row[k] = i < p.n ? row_at[i] : 0;
+        row[k] = i < count ? row_at[i] : 0;
         before[k] = 0;
     }
 #pragma unroll 4
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, R
 #pragma unroll
     for (int k = 0; k < R; k++) {
         const uint32_t i = first + mine + k;
-        if (share == 0 && i < p.n && i % 4)                        // but for the record itself and its four's later ones
+        if (share == 0 && i < count && i % 4)                        // but for the record itself and its four's later ones
             for (uint32_t j = i; j <= (i | 3); j++) before[k] -= row_at[j] == row[k];
         atomicAdd(&rank[mine + k], before[k]);
     }
@@ -432,8 +433,59 @@ __global__ __launch_bounds__(1024) void k_rows_rank(SortPass p, uint32_t part, R
 #pragma unroll
     for (int k = 0; k < R; k++) {
         const uint32_t i = first + mine + k;
-        if (i < p.n) p.out[rank[mine + k]] = {row[k], i};
+        if (i >= count) continue;
+        const uint32_t to = base + rank[mine + k];
+        if constexpr (TILE == kRankMost) {
+            p.out[to] = {row[k], i};
+        } else {
+            uint32_t* const rows = reinterpret_cast<uint32_t*>(p.out);                 // for k_rows_merge
+            rows[to] = row[k];
+            rows[p.n + to] = base + i;
+        }
     }
+}
+
+// Up to kMergeMost records: tiles of kMergeTile sorted as above, then each record's place is its own in its
+// tile and, by binary search in LDS, what the other tiles have below it (equal rows of earlier tiles too).
+// Two launches, bound by their latency. Sums of 64 columns: 8192 records 15.1 us, 20.1 by digits, 16384 16.0
+// and 22.2, 32768 21.9 and 27.6 (in tiles of 512 14.4, 16.1, 23.4, of 2048 16.7, 17.6, 26.6).
+constexpr uint32_t kMergeMost = 32768;
+constexpr uint32_t kMergeTile = 1024;
+
+__global__ __launch_bounds__(1024) void k_rows_merge(SortPass p, uint32_t part) {
+    __shared__ uint4 rows_at[kMergeMost / 4];
+    __shared__ uint32_t rank[kMergeMost / 256];
+    const uint32_t* const rows = reinterpret_cast<const uint32_t*>(p.in);              // n rows, then their records
+    const uint32_t* const row_at = reinterpret_cast<const uint32_t*>(rows_at);
+    const uint32_t first = blockIdx.x * part;
+    if (threadIdx.x < part) rank[threadIdx.x] = 0;
+    constexpr int U = 4;                                           // reads in flight
+    for (uint32_t c0 = threadIdx.x; c0 * 4 < p.n; c0 += 1024 * U) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) r[u] = reinterpret_cast<const uint4*>(rows)[min(c0 + u * 1024, (p.n - 1) / 4)];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if ((c0 + u * 1024) * 4 < p.n) rows_at[c0 + u * 1024] = r[u];
+    }
+    __syncthreads();
+    const uint32_t tiles = (p.n + kMergeTile - 1) / kMergeTile;
+    for (uint32_t x = threadIdx.x; x < part * tiles; x += 1024) {
+        const uint32_t mine = x % part, tile = x / part, i = first + mine, base = tile * kMergeTile;
+        if (i >= p.n) continue;
+        uint32_t below = i - base;
+        if (tile != i / kMergeTile) {
+            const uint32_t limit = row_at[i] + (base < i), count = min(kMergeTile, p.n - base);
+            below = 0;
+#pragma unroll
+            for (uint32_t step = kMergeTile; step; step /= 2)
+                if (below + step <= count && row_at[base + below + step - 1] < limit) below += step;
+        }
+        atomicAdd(&rank[mine], below);
+    }
+    __syncthreads();
+    const uint32_t i = first + threadIdx.x;
+    if (threadIdx.x < part && i < p.n) p.out[rank[threadIdx.x]] = {row_at[i], rows[p.n + i]};
 }
 
 // Sum: a group of LPR lanes (8 elements each) takes a tile of K neighbours of the sorted records. A row
@@ -825,11 +877,12 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
         return hipGetLastError();
     }); }); });
 }
+enum RowSort { kRanked, kMerged, kDigits };
 // How a batch of adds runs, and its workspace: two lists of (row, record), the digit counts, and the
 // parts of rows that reach past a group's records.
 struct AddPlan {
     uint32_t few;                            // k_rows_add_few for at most so many records, 0: sorted
-    bool ranked;                             // k_rows_rank, not a sort by digits
+    RowSort sort;
     uint32_t bits, passes, ipt, tiles;       // sort: bits of a digit, passes, records a thread takes, tiles
     uint32_t lanes, chunks, k, groups;       // sum: lanes of a group, its column chunks, records, groups
     uint32_t pitch;
@@ -841,11 +894,11 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     p.few = n <= 512 && blocks <= 4096 ? 512 : n <= 1024 && blocks <= 2048 ? 1024 : 0;
     if (p.few) return p;
     const uint32_t key_bits = 32 - __builtin_clz(uint32_t(rows) | 1);     // keys 0 .. rows
-    p.ranked = n <= kRankMost;
+    p.sort = n <= kRankMost ? kRanked : n <= kMergeMost ? kMerged : kDigits;
     p.passes = (key_bits + kSortBits - 1) / kSortBits;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    // (tiles of 512, 1024, 2048 and 4096 records: see above kSortThreads)
-    p.ipt = n <= 16384 ? 1 : n <= (1 << 18) ? 2 : n <= (1 << 20) ? 4 : 8;
+    // (tiles of 1024, 2048 and 4096 records: see above kSortThreads)
+    p.ipt = n <= (1 << 18) ? 2 : n <= (1 << 20) ? 4 : 8;
     p.tiles = uint32_t((n + p.ipt * kSortThreads - 1) / (p.ipt * kSortThreads));
     const uint32_t cols = (row_len + kChunk - 1) / kChunk;
     p.lanes = cols > 32 ? 64 : cols > 16 ? 32 : cols > 8 ? 16 : 8;
@@ -860,8 +913,8 @@ AddPlan add_plan(uint64_t rows, uint32_t row_len, uint64_t n) {
     uint64_t at = 0;
     auto take = [&at](uint64_t bytes) { const uint64_t o = at; at += (bytes + 255) & ~uint64_t(255); return o; };
     p.rec[0] = take(n * sizeof(uint2));
-    p.rec[1] = take(!p.ranked && p.passes > 1 ? n * sizeof(uint2) : 0);
-    p.hist = take(p.ranked ? 0 : (uint64_t(p.tiles) + 1) << p.bits << 2);
+    p.rec[1] = take(p.sort == kMerged || (p.sort == kDigits && p.passes > 1) ? n * sizeof(uint2) : 0);
+    p.hist = take(p.sort != kDigits ? 0 : (uint64_t(p.tiles) + 1) << p.bits << 2);
     p.joins = take((uint64_t(p.groups) + 1) * 4);
     p.first = take(uint64_t(p.groups) * p.pitch * 4);
     p.last = take(uint64_t(p.groups) * p.pitch * 4);
@@ -873,12 +926,23 @@ template <int IW>
 hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b, uint8_t* work, uint32_t* err, hipStream_t s,
                         const uint2** sorted) {
     const uint2* in = nullptr;
-    if (p.ranked) {
+    const uint32_t n = uint32_t(b.n);
+    uint32_t* const joins = reinterpret_cast<uint32_t*>(work + p.joins);
+    if (p.sort != kDigits) {
         uint2* const a = reinterpret_cast<uint2*>(work + p.rec[0]);
-        const SortPass q = {nullptr, a, nullptr, uint32_t(b.n), 0, 0, 1, false, reinterpret_cast<uint32_t*>(work + p.joins)};
-        const uint32_t part = std::max<uint32_t>(16, uint32_t(b.n + 511) / 512 * 2);       // 256 blocks
-        hipLaunchKernelGGL((k_rows_rank<IW>), dim3((uint32_t(b.n) + part - 1) / part), dim3(1024), 0, s, q, part, b, tab, err);
         *sorted = a;
+        if (p.sort == kRanked) {
+            const uint32_t part = std::max<uint32_t>(16, (n + 511) / 512 * 2);         // 256 blocks
+            hipLaunchKernelGGL((k_rows_rank<IW, kRankMost>), dim3((n + part - 1) / part), dim3(1024), 0, s,
+                               SortPass{nullptr, a, nullptr, n, 0, 0, 1, false, joins}, part, b, tab, err);
+            return hipGetLastError();
+        }
+        uint2* const t = reinterpret_cast<uint2*>(work + p.rec[1]);
+        const uint32_t part = (n + 255) / 256;
+        hipLaunchKernelGGL((k_rows_rank<IW, kMergeTile>), dim3((n + 63) / 64), dim3(1024), 0, s,
+                           SortPass{nullptr, t, nullptr, n, 0, 0, 1, false, joins}, 64u, b, tab, err);
+        hipLaunchKernelGGL(k_rows_merge, dim3((n + part - 1) / part), dim3(1024), 0, s,
+                           SortPass{t, a, nullptr, n, 0, 0, 1, false, joins}, part);
         return hipGetLastError();
     }
     for (uint32_t i = 0; i < p.passes; i++) {
@@ -891,8 +955,7 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
             if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(1024), 0, s, q);
             hipLaunchKernelGGL((k_rows_place<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
         };
-        if (p.ipt == 1) go(std::integral_constant<int, 1>{});
-        else if (p.ipt == 2) go(std::integral_constant<int, 2>{});
+        if (p.ipt == 2) go(std::integral_constant<int, 2>{});
         else if (p.ipt == 4) go(std::integral_constant<int, 4>{});
         else go(std::integral_constant<int, 8>{});
         in = out;

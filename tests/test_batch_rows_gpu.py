@@ -191,10 +191,10 @@ def test_add_large(lam, world, n, rows, width, how):
     check_close(a.local_rows(), exact, bound)
 
 
-@pytest.mark.parametrize("n", [16384, 16385, 65536, 65537, 262143, 262145, 1 << 20, (1 << 20) + 1, 3000001])
+@pytest.mark.parametrize("n", [1025, 4097, 6143, 6144, 6145, 7169, 32767, 32768, 32769, 65536, 65537, 262143, 262145, 1 << 20, (1 << 20) + 1, 3000001])
 @pytest.mark.parametrize("rows", [700, 3000017])
 def test_add_many_records(lam, world, n, rows):
-    """Sort tiles of each size, few and many of them. Whole numbers: the sums are exact (below 2^24: a row
+    """Sorted by each means, tiles of each size, few and many of them. Whole numbers: the sums are exact (below 2^24: a row
     has at most 16 n / rows + 2^16 records of at most 8)."""
     g = gen(n)
     a = lam.RowArray(world.team(), rows, 2)
