@@ -492,8 +492,8 @@ __global__ __launch_bounds__(1024) void k_rows_merge(SortPass p, uint32_t part) 
 // whose records begin in the tile and end there or in the next one is summed by this group alone and
 // added to the table at once. Only longer runs are cut: their parts go to `last` (the tile in which
 // they begin) and `first` (every later one), and k_rows_join adds them up. Every value is read once and
-// every named row read and written once: 131072 bf16 records of 4096 into f32 take 448 us here (4.9 TB/s
-// of the 2.2 GB that must move) of 502 in all.
+// every named row read and written once: 131072 bf16 records of 4096 into f32 take 443 us here (4.9 TB/s
+// of the 2.2 GB that must move) of 496 in all.
 struct SumArgs {
     const uint2* rec;     // sorted (row, record)
     float* first;         // [tiles][pitch]
