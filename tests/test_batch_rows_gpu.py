@@ -622,6 +622,31 @@ def test_decode_steps(lam, world):
     cache.wait_all()
 
 
+def test_captured_sums_of_every_size(lam, world):
+    """Sums of few to many records, one after the other in one graph; whole numbers, so that they are exact."""
+    g = gen(77)
+    sizes = [300, 900, 5003, 7001, 32768, 40000, 300001]
+    tab = lam.RowArray(world.team(), 4099, 24)
+    idx = [torch.zeros(n, dtype=torch.int64, device="cuda") for n in sizes]
+    val = [torch.zeros(n, 24, device="cuda") for n in sizes]
+    tab.batch_add_rows(idx[0], val[0]).block()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i, v in zip(idx, val):
+            tab.batch_add_rows(i, v).spawn()
+    exp = torch.zeros(4099, 24, dtype=torch.float64)
+    for r in range(3):
+        for i, v in zip(idx, val):
+            i.copy_(indices(g, i.numel(), 4099, "skewed" if r % 2 else "any"))
+            v.copy_(torch.randint(-8, 9, v.shape, generator=g).float())
+            exp.index_add_(0, i.cpu(), v.double().cpu())
+        graph.replay()
+        other = lam.RowArray(world.team(), 4099, 24)                # eager work between the replays
+        other.batch_add_rows(idx[3], val[3]).block()
+        torch.cuda.synchronize()
+        assert torch.equal(tab.local_rows().double().cpu(), exp), r
+
+
 def test_two_graphs_at_once(lam, world):
     """Two captured gradients and cache writes, each with its own workspace, replayed on two streams."""
     g = gen(21)
