@@ -271,11 +271,14 @@ class RowArray:
         return s
 
     def _claims(self, k, stream):
-        """The table with the words that stores of many records need: made once, but inside a capture
-        the graph gets its own (their clearing is part of the graph and has not run yet)."""
+        """The table with the words that stores of many records need: made once. Inside a capture the graph
+        gets its own (a replay clears them first, and may come when the array is gone)."""
         t = self._table
+        capturing = k.capturing()
+        if t.claims is not None and not capturing:
+            return t
         claims = torch.zeros(t.rows, dtype=torch.int32, device=k.device)
-        if k.capturing():
+        if capturing:
             return _Table(t.data, t.scales, claims, t.rows, t.row_len, t.rtype, t.group)
         t.claims, t.c.claims = claims, claims.data_ptr()
         self._streams = {stream}          # other streams are told of it when they next use the array
@@ -381,7 +384,7 @@ class RowArray:
         if add:
             k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride, stream)
         else:
-            table = self._table if n <= SCAN or self._table.claims is not None else self._claims(k, stream)
+            table = self._table if n <= SCAN else self._claims(k, stream)
             k.rows_store(table, idx, n, pad, vals, rt.code, stride, stream)
         return None
 

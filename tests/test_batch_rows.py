@@ -211,6 +211,34 @@ def test_c_entry_refusals(capi, lam):
         assert add(table(), n=big, work=p + 4, nbytes=need) == 7
 
 
+def test_captured_store_has_its_own_claims(lam):
+    """A store of many records that is captured into a graph takes claim words of its own, also where an
+    eager store has made the array's: a replay may come when the array is gone."""
+    seen = []
+
+    class Kernels(CpuRowKernels):
+        graph = False
+
+        def capturing(self):
+            return self.graph
+
+        def rows_store(self, table, *a):
+            seen.append(table.claims)
+            super().rows_store(table, *a)
+
+    team = lam.LamellarWorldBuilder().with_kernels(Kernels).build().team()
+    a = lam.RowArray(team, 7, 2)
+    i, v = torch.arange(1025) % 7, torch.ones(1025, 2)
+    a.batch_store_rows(i, v).block()
+    for graph in (True, True, False):
+        team.kernels.graph = graph
+        a.batch_store_rows(i, v).spawn()
+    team.kernels.graph = False
+    own = seen[0]
+    assert a._table.claims is own and own.numel() == 7 and seen[3] is own
+    assert all(c is not own and c.numel() == 7 and not c.any() for c in seen[1:3]) and seen[1] is not seen[2]
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)

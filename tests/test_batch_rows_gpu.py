@@ -682,6 +682,43 @@ def test_two_graphs_at_once(lam, world):
     world.wait_all()
 
 
+def test_captured_on_a_warmed_array(lam, world):
+    """Stores of many records, eager first, then captured, on the same array; replays on new inputs with
+    eager stores between them, and one when the array is gone and its memory used otherwise."""
+    g = gen(31)
+    n, rows, width, group = 1500, 600, 40, 8
+    mem, scales = torch.zeros(rows, width, dtype=torch.uint8).cuda(), torch.zeros(rows, width // group).cuda()
+    a = lam.RowArray.from_tensor(world.team(), mem, scales=scales, dtype="i8")
+    idx, vals = indices(g, n, rows, "any").cuda(), torch.randn(n, width, generator=g).cuda()
+    a.batch_store_rows(idx, vals).block()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.batch_store_rows(idx, vals).spawn()
+
+    def check(i, v):
+        last = ref.last_records(i, rows)
+        at, t = torch.tensor(list(last)), torch.tensor([last[r] for r in last])
+        codes, exp = ref.quantise(v[t], "i8", group)
+        assert torch.equal(scales.cpu()[at], exp) and torch.equal(mem.cpu()[at], codes)
+
+    for r in range(4):
+        if r == 3:
+            torch.cuda.synchronize()
+            del a
+            other = [torch.full((rows,), 1 << 30, dtype=torch.int32, device="cuda") for _ in range(8)]
+        i, v = indices(g, n, rows, "skewed" if r % 2 else "any"), torch.randn(n, width, generator=g)
+        idx.copy_(i)
+        vals.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(i, v)
+        if r < 3:
+            i, v = indices(g, 2000, rows, "any"), torch.randn(2000, width, generator=g)
+            a.batch_store_rows(i.cuda(), v.cuda()).block()
+            check(i, v)
+    assert all((o == 1 << 30).all() for o in other)
+
+
 @pytest.mark.parametrize("width", [1 << 18, (1 << 18) - 1, (1 << 18) - 8])
 def test_longest_rows(lam, world, width):
     g = gen(width)
