@@ -525,7 +525,7 @@ typedef struct {
     uint32_t type;       /* lmr_row_type_t */
     uint32_t group;      /* 8-bit types: elements per scale, divides row_len */
 } lmr_rows_t;
-/* out[t, :] = scale * table[idx[t], :] */
+/* out[t, :] = scale * table[idx[t], :] (8-bit tables: scale * (code * its group's scale)) */
 lmr_status_t lmr_rows_load(lmr_ctx_t* ctx, const lmr_rows_t* table, const void* d_idx, uint32_t index_size, uint64_t n,
                            int has_pad, int64_t pad, float scale, void* d_out, uint32_t out_type, uint64_t out_stride,
                            lmr_stream_t stream);

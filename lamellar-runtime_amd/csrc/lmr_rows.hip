@@ -102,9 +102,13 @@ __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* 
                 }
             }
         }
-        float m = b.scale;
-        if constexpr (is_code<T>::v && GA) m *= sc[u];
-        if (!live[u]) m = 0.f;                           // (times a chunk of zeros)
+        // (the code's product first: scale times a group's scale may leave f32's range where the result does not)
+        if constexpr (is_code<T>::v && GA) {
+            const float s = live[u] ? sc[u] : 0.f;
+#pragma unroll
+            for (int i = 0; i < kChunk; i++) v[i] *= s;
+        }
+        const float m = live[u] ? b.scale : 0.f;         // (times a chunk of zeros)
 #pragma unroll
         for (int i = 0; i < kChunk; i++) v[i] *= m;
         O* p = out + uint64_t(t[u]) * b.stride;

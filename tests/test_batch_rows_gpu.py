@@ -759,3 +759,20 @@ def test_batches_past_32_bits(lam, world):
     got[-1].fill_(1.0)
     q.batch_store_rows(i, got).block()
     assert torch.equal(q.batch_load_rows([rows - 1], out_dtype="f32").block().cpu(), torch.ones(1, width))
+
+
+@pytest.mark.parametrize("kind", CODES)
+def test_load_codes_far_scales(lam, world, kind):
+    """scale * (code * s) where scale * s would leave f32's range (or its normal numbers) although the result
+    does not, zero codes among them: the same bits for groups that are a multiple of 8 and others."""
+    codes = torch.tensor([0.0, 1.0, -2.0, 3.0, 120.0, 0.0, -0.0, 96.0] * 3)
+    c = codes.to(torch.int8 if kind == "i8" else torch.float8_e4m3fn).view(torch.uint8).expand(4, -1).contiguous()
+    s = torch.tensor([1e30, 1e-30, 2.0 ** -126, 3.0])
+    for scale in (1e10, 1e-10, 2.0 ** -120, 1.0):
+        got = []
+        for group in (24, 8, 12, 1):
+            a = lam.RowArray.from_tensor(world.team(), c.cuda(), scales=s[:, None].expand(4, 24 // group).contiguous().cuda(), dtype=kind)
+            got.append(a.batch_load_rows([0, 1, 2, 3], scale=scale, out_dtype="f32").block().cpu())
+        exp = codes * s[:, None] * scale                 # two f32 roundings, in this order
+        assert all(torch.equal(x, exp) for x in got), (scale, [(x != exp).nonzero().tolist() for x in got])
+        assert not exp[:, 0].any() and torch.isfinite(exp[1:]).all()
