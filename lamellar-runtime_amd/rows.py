@@ -80,20 +80,33 @@ def _value_type(t) -> RowType:
     return r
 
 
+def _again(e):
+    """The same exception without its traceback, which would hold the batch's tensors."""
+    c = type(e).__new__(type(e), *e.args)
+    c.__dict__.update(e.__dict__)
+    return c
+
+
 class RowsHandle(_Handle):
     """A batch of rows: spawn() enqueues it, value() its result without waiting, block() the result
     once the device has finished (raising its errors)."""
 
     def __init__(self, array, launch):
         self._array, self._launch = array, launch
-        self._res = None
+        self._res = self._error = None
         self._launched = False
 
     def spawn(self):
         if not self._launched:
             self._launched = True
             launch, self._launch = self._launch, None      # its tensors live as long as the stream needs them
-            self._res = launch()
+            try:
+                self._res = launch()
+            except BaseException as e:
+                self._error = _again(e)
+                raise
+        elif self._error is not None:                      # it has no result, however often it is asked
+            raise _again(self._error)
         return self
 
     def value(self):

@@ -4,6 +4,7 @@ import ctypes
 import os
 import sys
 import tempfile
+import warnings
 
 import numpy as np
 import pytest
@@ -237,6 +238,22 @@ def test_captured_store_has_its_own_claims(lam):
     own = seen[0]
     assert a._table.claims is own and own.numel() == 7 and seen[3] is own
     assert all(c is not own and c.numel() == 7 and not c.any() for c in seen[1:3]) and seen[1] is not seen[2]
+
+
+def test_refused_handles_stay_refused(lam, team):
+    """A handle whose batch was turned down raises every time it is asked, and gives no result."""
+    a = lam.RowArray(team, 10, 6)
+    for h in (a.batch_add_rows([0, 1, 2], torch.ones(2, 6)), a.batch_store_rows([0, 1, 2], torch.ones(2, 6)),
+              a.batch_load_rows([0, 1, 2], out=torch.empty(2, 6))):
+        for call in (h.spawn, h.value, h.block, h.spawn):
+            refused(lam, LENGTH, call)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")               # it was spawned: nothing to warn of
+            del h, call
+    bad = a.batch_load_rows(torch.ones(3))
+    refused(lam, INVALID, bad.value)
+    refused(lam, INVALID, bad.block)
+    assert not a.local_rows().any()
 
 
 # ------------------------------------------------------------------ several PEs
