@@ -21,6 +21,9 @@ Indices are integers of any shape: torch tensors (int32 and int64 are read as th
 lists, one number. Values are torch tensors of f32, f16 or bf16; host sequences are taken as f32. A
 batch has at most 2^25 records and 2^36 elements.
 
+A lookup is not recorded by autograd: its gradient is the caller's batch_add_rows. Batches write a tensor
+that the caller gave (from_tensor, out) in place and raise its version, as torch's in-place operations do.
+
 Handles are lazy, as the element arrays': spawn() enqueues the batch on torch's current stream,
 value() gives its result for work ordered after it on that stream, block() waits and raises what the
 batch found wrong. A spawned batch reads its inputs in stream order, so later work on the stream may
@@ -350,7 +353,8 @@ class RowArray:
         n, shape = idx.numel(), (*shape, self.row_len)
         alone = not self._distributed
         stride = self.row_len
-        if out is None:
+        fresh = out is None
+        if fresh:
             rows = out = torch.empty(shape, dtype=rt.torch, device=k.device)
             if len(shape) != 2:
                 rows = out.view(n, self.row_len)
@@ -363,6 +367,8 @@ class RowArray:
             self._exchange_load(k, idx, scale, rt, pad, rows, n)
         elif n:
             k.rows_load(self._table, idx, n, pad, scale, rows, rt.code, stride, stream)
+        if not fresh:
+            _written(out)
         return out
 
     def _out_rows(self, k, out, shape, n):
@@ -395,10 +401,14 @@ class RowArray:
             return None
         stride = vals.stride(0) if n > 1 else self.row_len
         if add:
-            k.rows_add(self._table, idx, n, pad, scale, vals, rt.code, stride, stream)
+            table = self._table
+            k.rows_add(table, idx, n, pad, scale, vals, rt.code, stride, stream)
         else:
             table = self._table if n <= SCAN else self._claims(k, stream)
             k.rows_store(table, idx, n, pad, vals, rt.code, stride, stream)
+        _written(table.data)
+        if table.scales is not None:
+            _written(table.scales)
         return None
 
     # Records travel to their rows' owner in input order (the stable pack), sources one after the
@@ -440,6 +450,11 @@ class RowArray:
     def _exchange_values(self, k, idx, vals, pad):
         mine, pos, sent, got = self._pack(k, idx, pad)
         return mine, _all_to_all(self.team, vals.index_select(0, pos), sent, got), None
+
+
+def _written(t):
+    """Tells autograd that t's memory was changed: what a backward pass has saved of it is no longer good."""
+    torch.autograd.graph.increment_version(t)
 
 
 def _device_of(x):

@@ -256,6 +256,48 @@ def test_refused_handles_stay_refused(lam, team):
     assert not a.local_rows().any()
 
 
+def test_writes_are_seen_by_autograd(lam):
+    """A batch that writes raises the version of what it wrote, so that a backward pass over a tensor saved
+    before it is refused, as after torch's own in-place operations; a lookup leaves the table's version."""
+
+    class Kernels(CpuRowKernels):                        # writes past torch, as the device does
+        def rows_load(self, table, idx, n, pad, scale, out, *a):
+            out.numpy()[:] = scale
+
+        def rows_add(self, table, *a):
+            table.data.numpy()[0] += 1
+
+        def rows_store(self, table, *a):
+            table.data.numpy()[0] = 5
+
+    team = lam.LamellarWorldBuilder().with_kernels(Kernels).build().team()
+    for write in ("batch_add_rows", "batch_store_rows"):
+        weight = torch.nn.Parameter(torch.ones(4, 3))
+        a = lam.RowArray.from_tensor(team, weight)
+        loss = (weight * weight).sum()
+        a.batch_load_rows([1, 2]).block()
+        loss.backward(retain_graph=True)
+        getattr(a, write)([0], torch.ones(1, 3)).block()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    codes, scales = torch.zeros(4, 6, dtype=torch.uint8), torch.ones(4, 2, requires_grad=True)
+    c = lam.RowArray.from_tensor(team, codes, scales=scales, dtype="i8")
+    loss, was = (scales * scales).sum(), codes._version
+    c.batch_store_rows([0], torch.ones(1, 6)).block()
+    assert codes._version > was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    out, w = torch.zeros(2, 3), torch.ones(2, 3, requires_grad=True)
+    loss = (w * out).sum()
+    a.batch_load_rows([1, 2], out=out).block()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        d = lam.RowArray(team, 4, 3)
+        d.batch_store_rows([0], torch.ones(1, 3)).block()
+        d.batch_load_rows([0], out=torch.empty(1, 3)).block()
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)
