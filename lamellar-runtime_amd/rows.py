@@ -300,7 +300,7 @@ class RowArray:
         self._streams = {stream}          # other streams are told of it when they next use the array
         return t
 
-    def _index(self, k, index):
+    def _index(self, k, index, pad):
         """(1-D index tensor of 4 or 8 bytes, the shape it had)."""
         if isinstance(index, Owned):
             index = index.value
@@ -312,13 +312,17 @@ class RowArray:
                 return index, shape
             if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
                 raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {index.dtype}")
-            return index_input(k, index)[1], shape
-        if isinstance(index, numbers.Integral):
-            return torch.tensor([int(index)], dtype=torch.int64, device=k.device), torch.Size([])
+            unsigned = index.dtype == torch.uint64
+            index = index_input(k, index)[1]
+            return _no_wrap(index, pad) if unsigned else index, shape
+        if isinstance(index, numbers.Integral) and type(index) is not bool:
+            i = int(index)
+            return torch.tensor([i if _fits(i) else _nowhere(pad)], dtype=torch.int64, device=k.device), torch.Size([])
         a = np.asarray(index)
         if a.size and a.dtype.kind not in "iu":
-            raise LamellarError(LmrStatus.INVALID, f"row indices are integers, not {a.dtype}")
-        return index_input(k, a.reshape(-1))[1], torch.Size(a.shape)
+            raise LamellarError(LmrStatus.INVALID, f"row indices are integers below 2^63, not {a.dtype}")
+        i = index_input(k, a.reshape(-1))[1]
+        return _no_wrap(i, pad) if a.dtype == np.uint64 else i, torch.Size(a.shape)
 
     def _values(self, k, vals, n):
         """(n x row_len tensor whose rows are contiguous, their type)."""
@@ -349,7 +353,7 @@ class RowArray:
 
     def _load(self, index, scale, rt, pad, out):
         k = self.team.kernels
-        idx, shape = self._index(k, index)
+        idx, shape = self._index(k, index, pad)
         n, shape = idx.numel(), (*shape, self.row_len)
         alone = not self._distributed
         stride = self.row_len
@@ -390,7 +394,7 @@ class RowArray:
 
     def _write(self, index, vals, scale, pad, add):
         k = self.team.kernels
-        idx, _ = self._index(k, index)
+        idx, _ = self._index(k, index, pad)
         n = idx.numel()
         vals, rt = self._values(k, vals, n)
         stream = self._on_stream(k)
@@ -465,17 +469,31 @@ def _device_of(x):
 def _scale(x):
     if type(x) is float:
         return x
-    if not isinstance(x, (numbers.Real, np.generic)):
+    if not isinstance(x, numbers.Real) or type(x) is bool:
         raise LamellarError(LmrStatus.INVALID, f"scale is a number, not {type(x).__name__}")
     return float(x)
 
 
+def _fits(i):
+    return -(1 << 63) <= i < 1 << 63
+
+
 def _pad(x):
-    if x is None or type(x) is int and -(1 << 63) <= x < 1 << 63:
+    if x is None or type(x) is int and _fits(x):
         return x
-    if not isinstance(x, numbers.Integral) or not -(1 << 63) <= int(x) < 1 << 63:
+    if not isinstance(x, numbers.Integral) or type(x) is bool or not _fits(int(x)):
         raise LamellarError(LmrStatus.INVALID, f"pad is an index, not {x!r}")
     return int(x)
+
+
+def _nowhere(pad):
+    """A number of 64 bits that is neither a row nor the pad."""
+    return -(1 << 63) if pad != -(1 << 63) else 1 - (1 << 63)
+
+
+def _no_wrap(i, pad):
+    """Unsigned indices read as signed ones: those of 2^63 and more name no row, whatever they look like."""
+    return torch.where(i < 0, _nowhere(pad), i)
 
 
 def _all_to_all(team, rows, sent, got):

@@ -298,6 +298,35 @@ def test_writes_are_seen_by_autograd(lam):
         d.batch_load_rows([0], out=torch.empty(1, 3)).block()
 
 
+def test_refused_numbers(lam, team):
+    """Truth values are no indices, pads or scales, alone or in a list; integers past 63 bits name no row, and
+    none of them is taken for another number (2^64 - 1 is not the pad -1)."""
+    a = lam.RowArray(team, 10, 6)
+    v = torch.ones(6)
+    for h in (a.batch_load_rows, lambda i, **k: a.batch_add_rows(i, v, **k), lambda i, **k: a.batch_store_rows(i, v, **k)):
+        for i in (True, np.bool_(True), [True], np.ones(1, dtype=bool), torch.tensor(True)):
+            refused(lam, INVALID, lambda: h(i).block())
+        for pad in (True, np.bool_(False), torch.tensor(1)):
+            refused(lam, INVALID, lambda: h([1], pad=pad).block())
+        top = (1 << 64) - 1
+        for i in (np.array([top], dtype=np.uint64), np.uint64(top), top, [top], -(1 << 63) - 1,
+                  torch.tensor([-1]).view(torch.uint64)):
+            for pad in (-1, -(1 << 63), None):
+                refused(lam, OOB, lambda: h(i, pad=pad).block())
+        a.local_rows().zero_()
+        for i in ([1 << 70], [1, 1 << 63]):              # lists that have no integer type
+            refused(lam, INVALID, lambda: h(i).block())
+    assert not a.local_rows().any()
+    for scale in (True, np.bool_(True), np.str_("2"), np.complex64(2), 1j):
+        refused(lam, INVALID, lambda: a.batch_load_rows([1], scale=scale).block())
+        refused(lam, INVALID, lambda: a.batch_add_rows([1], v, scale=scale).block())
+    a.batch_add_rows(np.uint64(3), v, scale=np.float16(0.5)).block()
+    a.batch_add_rows(np.array([3], dtype=np.uint64), v, scale=2).block()
+    a.batch_add_rows([3, np.int8(3), -1], v, pad=np.int64(-1)).block()
+    a.batch_add_rows(torch.tensor([3], dtype=torch.uint16), v).block()
+    assert (a.local_rows()[3] == 5.5).all() and int((a.local_rows() != 0).sum()) == 6
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)
