@@ -19,7 +19,7 @@ PE that names the row when several do.
 
 Indices are integers of any shape: torch tensors (int32 and int64 are read as they are), numpy arrays,
 lists, one number. Values are torch tensors of f32, f16 or bf16; host sequences are taken as f32. A
-batch has at most 2^25 records and 2^36 elements.
+batch has at most 2^25 records and 2^36 elements, at a PE that sends them and at one that gets them.
 
 A lookup is not recorded by autograd: its gradient is the caller's batch_add_rows. Batches write a tensor
 that the caller gave (from_tensor, out) in place and raise its version, as torch's in-place operations do.
@@ -65,6 +65,8 @@ _BY_TORCH = {t.torch: t for t in ROW_TYPES.values()}
 _VALUES = {k: t for t in ROW_TYPES.values() if not t.is_code for k in (t.name, t.torch)}
 MAX_ROW_LEN = 1 << 18                     # LMR_ROW_MAX_LEN
 MAX_ROWS = 0xFFFFFFF0                     # LMR_ROWS_MAX, of one PE
+MAX_BATCH = 1 << 25                       # LMR_ROW_MAX_BATCH, records that one PE sends or gets
+MAX_VALUES = 1 << 36                      # LMR_ROW_MAX_VALUES, their elements
 SCAN = 1024                               # LMR_ROW_SCAN: stores of more records use claims
 _INT = (torch.int64, torch.int32)
 
@@ -417,7 +419,8 @@ class RowArray:
 
     # Records travel to their rows' owner in input order (the stable pack), sources one after the
     # other: the owner sees one batch in an order that every run repeats. The counts are read on the
-    # host, so a batch over several PEs waits for its pack.
+    # host, so a batch over several PEs waits for its pack. Every PE gets the counts of all, so that a
+    # batch too large for one of them is turned down by all of them, before its records travel.
     def _pack(self, k, idx, pad):
         gidx = idx.to(torch.int64)
         kept = None
@@ -427,11 +430,15 @@ class RowArray:
         n = int(gidx.numel())
         loc, _, pos, counts = k.pack(self.layout, gidx, n, None, DTYPES["u8"], 8)
         sent = [int(c) for c in counts.cpu().tolist()]
+        every = _all_gather(self.team, [idx.numel(), *sent])
+        for p in range(len(sent)):
+            most = max(every[p][0], sum(e[1 + p] for e in every))
+            if most > MAX_BATCH or most * self.row_len > MAX_VALUES:
+                raise LamellarError(LmrStatus.INVALID, f"PE {p} would send or get {most} rows of {self.row_len} (at most "
+                                                       f"{MAX_BATCH}, of {MAX_VALUES} elements)")
+        got = [e[1 + self.team.my_pe()] for e in every]
         m = sum(sent)                                   # an index out of bounds is dropped there
         pos = pos[:m].to(torch.int64)
-        got = _all_to_all(self.team, torch.tensor(sent, dtype=torch.int64, device=k.device).view(-1, 1),
-                          [1] * len(sent), [1] * len(sent))
-        got = [int(c) for c in got.view(-1).cpu().tolist()]
         loc = loc.view(torch.int64)[:m].view(-1, 1) if m else gidx[:0].view(0, 1)
         return _all_to_all(self.team, loc, sent, got).view(-1), (pos if kept is None else kept[pos]), sent, got
 
@@ -494,6 +501,15 @@ def _nowhere(pad):
 def _no_wrap(i, pad):
     """Unsigned indices read as signed ones: those of 2^63 and more name no row, whatever they look like."""
     return torch.where(i < 0, _nowhere(pad), i)
+
+
+def _all_gather(team, numbers_of_this):
+    """Every PE's list of whole numbers, equally many from each, in PE order."""
+    dev = team.kernels.device if dist.get_backend(team.group) == "nccl" else torch.device("cpu")
+    mine = torch.tensor(numbers_of_this, dtype=torch.int64).to(dev)
+    every = torch.empty(team.num_pes() * mine.numel(), dtype=torch.int64, device=dev)
+    dist.all_gather_into_tensor(every, mine, group=team.group)
+    return every.cpu().view(team.num_pes(), -1).tolist()
 
 
 def _all_to_all(team, rows, sent, got):

@@ -4,6 +4,7 @@ import ctypes
 import os
 import sys
 import tempfile
+import time
 import warnings
 
 import numpy as np
@@ -410,3 +411,63 @@ def test_exchange_gloo(ws, dist_kind):
         assert int(r["oob"]) == (2 if p == 0 else 0)
         assert torch.equal(r["oob_rows"][0], torch.zeros(width) if p == 0 else stored[1])
         assert (r["five"] == ws).all()
+
+
+def _limit_worker(rank, ws, port, outdir):
+    sys.path.insert(0, ROOT)
+    sys.path.insert(0, os.path.join(ROOT, "tests"))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(ws), LOCAL_RANK=str(rank))
+    from _lamellar_bootstrap import load_package
+    lam = load_package()
+    from lamellar_runtime_amd import rows as rows_module
+    from test_batch_rows import CpuRowKernels
+
+    class Kernels(CpuRowKernels):                        # the device's limits, lowered
+        def _check(self, table, n):
+            if n > 20 or n * table.row_len > 100:
+                raise lam.LamellarError(1, "too many")
+
+        def rows_load(self, table, idx, n, *a):
+            self._check(table, n)
+            super().rows_load(table, idx, n, *a)
+
+        def rows_add(self, table, idx, n, *a):
+            self._check(table, n)
+            super().rows_add(table, idx, n, *a)
+
+        def rows_store(self, table, idx, n, *a):
+            self._check(table, n)
+            super().rows_store(table, idx, n, *a)
+
+    rows_module.MAX_BATCH, rows_module.MAX_VALUES = 20, 100
+    team, res = lam.LamellarWorldBuilder().with_kernels(Kernels).build().team(), []
+    for width, n in ((2, [11, 11]), (8, [7, 6]), (2, [21, 0]), (2, [11, 9])):
+        a = lam.RowArray(team, 10, width)
+        i = torch.full((n[rank],), 2)                    # all of PE 0's
+        spread = i.clone() if n[1] else torch.arange(n[rank]) % 10
+        for h in (a.batch_load_rows(spread), a.batch_add_rows(spread, torch.ones(width)), a.batch_store_rows(spread, torch.ones(width))):
+            try:
+                h.block()
+                res.append(0)
+            except lam.LamellarError as e:
+                res.append(int(e.status))
+        team.barrier()
+    np.savez(os.path.join(outdir, f"pe{rank}.npz"), res=np.array(res))
+    torch.distributed.barrier()
+    torch.distributed.destroy_process_group()
+
+
+def test_exchange_limits():
+    """A batch that would be too large for one PE is turned down by every PE, none waits for another."""
+    with tempfile.TemporaryDirectory() as d:
+        ctx = mp.spawn(_limit_worker, args=(2, 30350 + os.getpid() % 200, d), nprocs=2, join=False)
+        try:
+            until = time.monotonic() + 60
+            while not ctx.join(timeout=1):
+                assert time.monotonic() < until, "a PE waits"
+        finally:
+            for p in ctx.processes:
+                if p.is_alive():
+                    p.kill()
+        for r in range(2):
+            assert np.load(os.path.join(d, f"pe{r}.npz"))["res"].tolist() == [1] * 9 + [0] * 3
