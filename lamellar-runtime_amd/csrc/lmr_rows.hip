@@ -16,6 +16,7 @@
 #include "lmr_internal.hpp"
 #include "lmr_rows.hpp"
 #include <algorithm>
+#include <tuple>
 
 namespace lmr {
 namespace {
@@ -833,6 +834,16 @@ __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, co
     }
 }
 
+// A launch and its own status: what hipGetLastError holds may be an earlier call's, for whoever asks there.
+template <typename... P, typename... A>
+hipError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, hipStream_t s, const A&... given) {
+    std::tuple<P...> args(static_cast<P>(given)...);
+    return std::apply([&](auto&... a) {
+        void* at[] = {&a...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), at, 0, s);
+    }, args);
+}
+
 bool is_float_type(uint32_t type) { return type <= LMR_ROW_BF16; }
 template <typename F>
 hipError_t by_value_type(uint32_t type, F&& f) {
@@ -870,15 +881,9 @@ hipError_t launch_load(const RowTable& tab, const RowBatch& b, void* out, uint32
         const bool four = chunks >= 2048ull * 256;
         const dim3 grid(unsigned(four ? (chunks + 1023) / 1024 : (chunks + 255) / 256));
         if constexpr (is_code<T>::v) {
-            if (!ga) {
-                if (four) hipLaunchKernelGGL((k_rows_load<T, O, IW, 4, false>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
-                else hipLaunchKernelGGL((k_rows_load<T, O, IW, 1, false>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
-                return hipGetLastError();
-            }
+            if (!ga) return launch(four ? k_rows_load<T, O, IW, 4, false> : k_rows_load<T, O, IW, 1, false>, grid, 256, s, tab, b, p, err, cpr, cpg);
         }
-        if (four) hipLaunchKernelGGL((k_rows_load<T, O, IW, 4, true>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
-        else hipLaunchKernelGGL((k_rows_load<T, O, IW, 1, true>), grid, dim3(256), 0, s, tab, b, p, err, cpr, cpg);
-        return hipGetLastError();
+        return launch(four ? k_rows_load<T, O, IW, 4, true> : k_rows_load<T, O, IW, 1, true>, grid, 256, s, tab, b, p, err, cpr, cpg);
     }); }); });
 }
 enum RowSort { kRanked, kMerged, kDigits };
@@ -937,17 +942,15 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
         *sorted = a;
         if (p.sort == kRanked) {
             const uint32_t part = std::max<uint32_t>(16, (n + 511) / 512 * 2);         // 256 blocks
-            hipLaunchKernelGGL((k_rows_rank<IW, kRankMost>), dim3((n + part - 1) / part), dim3(1024), 0, s,
-                               SortPass{nullptr, a, nullptr, n, 0, 0, 1, false, joins}, part, b, tab, err);
-            return hipGetLastError();
+            return launch(k_rows_rank<IW, kRankMost>, dim3((n + part - 1) / part), 1024, s,
+                          SortPass{nullptr, a, nullptr, n, 0, 0, 1, false, joins}, part, b, tab, err);
         }
         uint2* const t = reinterpret_cast<uint2*>(work + p.rec[1]);
         const uint32_t part = (n + 255) / 256;
-        hipLaunchKernelGGL((k_rows_rank<IW, kMergeTile>), dim3((n + 63) / 64), dim3(1024), 0, s,
-                           SortPass{nullptr, t, nullptr, n, 0, 0, 1, false, joins}, 64u, b, tab, err);
-        hipLaunchKernelGGL(k_rows_merge, dim3((n + part - 1) / part), dim3(1024), 0, s,
-                           SortPass{t, a, nullptr, n, 0, 0, 1, false, joins}, part);
-        return hipGetLastError();
+        const hipError_t e = launch(k_rows_rank<IW, kMergeTile>, dim3((n + 63) / 64), 1024, s,
+                                    SortPass{nullptr, t, nullptr, n, 0, 0, 1, false, joins}, 64u, b, tab, err);
+        if (e != hipSuccess) return e;
+        return launch(k_rows_merge, dim3((n + part - 1) / part), 1024, s, SortPass{t, a, nullptr, n, 0, 0, 1, false, joins}, part);
     }
     for (uint32_t i = 0; i < p.passes; i++) {
         uint2* out = reinterpret_cast<uint2*>(work + p.rec[i & 1]);
@@ -955,17 +958,17 @@ hipError_t sort_records(const AddPlan& p, const RowTable& tab, const RowBatch& b
                       reinterpret_cast<uint32_t*>(work + p.joins)};
         auto go = [&](auto ipt) {
             constexpr int IPT = decltype(ipt)::value;
-            hipLaunchKernelGGL((k_rows_count<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
-            if (q.summed) hipLaunchKernelGGL(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), dim3(1024), 0, s, q);
-            hipLaunchKernelGGL((k_rows_place<IW, IPT>), dim3(p.tiles), dim3(kSortThreads), 0, s, q, b, tab, err);
+            hipError_t e = launch(k_rows_count<IW, IPT>, dim3(p.tiles), kSortThreads, s, q, b, tab, err);
+            if (e == hipSuccess && q.summed) e = launch(k_rows_prefix, dim3(((1u << p.bits) + 63) / 64), 1024, s, q);
+            return e != hipSuccess ? e : launch(k_rows_place<IW, IPT>, dim3(p.tiles), kSortThreads, s, q, b, tab, err);
         };
-        if (p.ipt == 2) go(std::integral_constant<int, 2>{});
-        else if (p.ipt == 4) go(std::integral_constant<int, 4>{});
-        else go(std::integral_constant<int, 8>{});
+        const hipError_t e = p.ipt == 2 ? go(std::integral_constant<int, 2>{}) : p.ipt == 4 ? go(std::integral_constant<int, 4>{})
+                                        : go(std::integral_constant<int, 8>{});
+        if (e != hipSuccess) return e;
         in = out;
     }
     *sorted = in;
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, void* work, uint32_t* err,
@@ -976,9 +979,8 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
             using V = decltype(v);
             const dim3 grid(unsigned(b.n), (tab.row_len + 511) / 512);
             const V* x = reinterpret_cast<const V*>(vals);
-            if (p.few == 512) hipLaunchKernelGGL((k_rows_add_few<decltype(t), V, decltype(iw)::value, 512>), grid, dim3(256), 0, s, tab, b, x, err);
-            else hipLaunchKernelGGL((k_rows_add_few<decltype(t), V, decltype(iw)::value, 1024>), grid, dim3(256), 0, s, tab, b, x, err);
-            return hipGetLastError();
+            return launch(p.few == 512 ? k_rows_add_few<decltype(t), V, decltype(iw)::value, 512>
+                                       : k_rows_add_few<decltype(t), V, decltype(iw)::value, 1024>, grid, 256, s, tab, b, x, err);
         }); }); });
     uint8_t* w = reinterpret_cast<uint8_t*>(work);
     const uint2* sorted = nullptr;
@@ -994,24 +996,22 @@ hipError_t launch_add(const RowTable& tab, const RowBatch& b, const void* vals, 
         using V = decltype(v);
         const V* x = reinterpret_cast<const V*>(vals);
         auto sum = [&](auto lanes, auto whole, auto u) {
-            hipLaunchKernelGGL((k_rows_sum<T, V, decltype(lanes)::value, decltype(whole)::value, decltype(u)::value>), dim3(blocks),
-                               dim3(256), 0, s, tab, b, x, a);
+            return launch(k_rows_sum<T, V, decltype(lanes)::value, decltype(whole)::value, decltype(u)::value>, dim3(blocks), 256, s, tab, b, x, a);
         };
         auto by_lanes = [&](auto whole, auto u) {
             switch (p.lanes) {
-            case 8: sum(std::integral_constant<int, 8>{}, whole, u); break;
-            case 16: sum(std::integral_constant<int, 16>{}, whole, u); break;
-            case 32: sum(std::integral_constant<int, 32>{}, whole, u); break;
-            default: sum(std::integral_constant<int, 64>{}, whole, u);
+            case 8: return sum(std::integral_constant<int, 8>{}, whole, u);
+            case 16: return sum(std::integral_constant<int, 16>{}, whole, u);
+            case 32: return sum(std::integral_constant<int, 32>{}, whole, u);
+            default: return sum(std::integral_constant<int, 64>{}, whole, u);
             }
         };
         // (131072 bf16 records of 4096: 514 us with 4 in flight, 504 with 8; ends of rows that are not whole cost
         // registers: 5003 of 1001 took 1.5 us longer with 8)
-        if (tab.row_len % kChunk) by_lanes(std::false_type{}, std::integral_constant<int, 4>{});
-        else if (p.k == 4) by_lanes(std::true_type{}, std::integral_constant<int, 4>{});
-        else by_lanes(std::true_type{}, std::integral_constant<int, 8>{});
-        hipLaunchKernelGGL((k_rows_join<T>), dim3(join_blocks), dim3(64 * kJoinWaves), 0, s, tab, b.scale, a, wide);
-        return hipGetLastError();
+        const hipError_t e = tab.row_len % kChunk ? by_lanes(std::false_type{}, std::integral_constant<int, 4>{})
+                             : p.k == 4           ? by_lanes(std::true_type{}, std::integral_constant<int, 4>{})
+                                                  : by_lanes(std::true_type{}, std::integral_constant<int, 8>{});
+        return e != hipSuccess ? e : launch(k_rows_join<T>, dim3(join_blocks), 64 * kJoinWaves, s, tab, b.scale, a, wide);
     }); });
 }
 hipError_t launch_store(const RowTable& tab, const RowBatch& b, const void* vals, uint32_t val_type, uint32_t* err, hipStream_t s) {
@@ -1028,20 +1028,21 @@ hipError_t launch_store(const RowTable& tab, const RowBatch& b, const void* vals
         using V = decltype(v);
         constexpr int IW = decltype(iw)::value;
         const V* x = reinterpret_cast<const V*>(vals);
-        if (how == kClaimed) hipLaunchKernelGGL((k_rows_claim<IW>), dim3(unsigned((b.n + 255) / 256)), dim3(256), 0, s, tab, b, err);
+        if (how == kClaimed) {
+            const hipError_t e = launch(k_rows_claim<IW>, dim3(unsigned((b.n + 255) / 256)), 256, s, tab, b, err);
+            if (e != hipSuccess) return e;
+        }
         auto go = [&](auto l) {
             constexpr int L = decltype(l)::value;
-            hipLaunchKernelGGL((k_rows_store<T, V, IW, L>), dim3(unsigned((b.n + 256 / L - 1) / (256 / L))), dim3(256), 0, s, tab, b, x,
-                               err, how, lpg);
+            return launch(k_rows_store<T, V, IW, L>, dim3(unsigned((b.n + 256 / L - 1) / (256 / L))), 256, s, tab, b, x, err, how, lpg);
         };
         switch (lanes) {
-        case 8: go(std::integral_constant<int, 8>{}); break;
-        case 16: go(std::integral_constant<int, 16>{}); break;
-        case 32: go(std::integral_constant<int, 32>{}); break;
-        case 64: go(std::integral_constant<int, 64>{}); break;
-        default: go(std::integral_constant<int, 256>{});
+        case 8: return go(std::integral_constant<int, 8>{});
+        case 16: return go(std::integral_constant<int, 16>{});
+        case 32: return go(std::integral_constant<int, 32>{});
+        case 64: return go(std::integral_constant<int, 64>{});
+        default: return go(std::integral_constant<int, 256>{});
         }
-        return hipGetLastError();
     }); }); });
 }
 
@@ -1112,11 +1113,15 @@ struct OnDevice {
     explicit OnDevice(int device) {
         ok = hipGetDevice(&was) == hipSuccess;
         if (ok && was != device) ok = moved = hipSetDevice(device) == hipSuccess;
-        (void)hipGetLastError();                             // what an earlier call left is not this one's
+        if (!ok) (void)hipGetLastError();
     }
     ~OnDevice() { if (moved) (void)hipSetDevice(was); }
 };
-lmr_status_t hip_status(hipError_t e) { return e == hipSuccess ? LMR_OK : LMR_E_HIP; }
+// (a failure is told by the status and not left in the runtime; an earlier call's error stays)
+lmr_status_t hip_status(hipError_t e) {
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e == hipSuccess ? LMR_OK : LMR_E_HIP;
+}
 
 }  // namespace
 }  // namespace lmr

@@ -776,3 +776,38 @@ def test_load_codes_far_scales(lam, world, kind):
         exp = codes * s[:, None] * scale                 # two f32 roundings, in this order
         assert all(torch.equal(x, exp) for x in got), (scale, [(x != exp).nonzero().tolist() for x in got])
         assert not exp[:, 0].any() and torch.isfinite(exp[1:]).all()
+
+
+def test_earlier_errors_are_left(lam, world):
+    """An error that an earlier call left in the runtime is no row batch's: the batch runs, and the error is still
+    there afterwards for whoever asks."""
+    import ctypes
+    path = next(x.split()[-1] for x in open("/proc/self/maps") if "libamdhip64" in x)
+    hip = ctypes.CDLL(path)                              # the library that is loaded already
+    k = world.team().kernels
+    a = lam.RowArray(world.team(), 3000, 16)
+    c = lam.RowArray(world.team(), 3000, 16, dtype="i8")
+    idx = {n: torch.arange(n, dtype=torch.int64, device="cuda") for n in (5, 2000)}
+    val = {n: torch.ones(n, 16, device="cuda") for n in idx}
+    c.batch_store_rows(idx[2000], val[2000]).block()     # its claims exist
+    work = torch.empty(k.lib.lmr_rows_add_workspace(a._table.ptr, 2000), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    hip.hipGetLastError()
+    assert hip.hipSetDevice(1 << 20) == 101              # refused on the host
+    kept = hip.hipGetDevice(ctypes.byref(ctypes.c_int())) == 0 and hip.hipPeekAtLastError() == 101
+    left = []
+    for n in (5, 2000):
+        i, v, s = idx[n].data_ptr(), val[n].data_ptr(), k.stream_id()
+        left.append(k.lib.lmr_rows_add(k.ctx, a._table.ptr, i, 8, n, 0, 0, 2.0, v, 0, 16, work.data_ptr(), work.numel(), s))
+        left.append(hip.hipPeekAtLastError())
+        left.append(k.lib.lmr_rows_store(k.ctx, c._table.ptr, i, 8, n, 0, 0, v, 0, 16, s))
+        left.append(hip.hipPeekAtLastError())
+        left.append(k.lib.lmr_rows_load(k.ctx, a._table.ptr, i, 8, n, 0, 0, 1.0, v, 0, 16, s))
+        left.append(hip.hipPeekAtLastError())
+    hip.hipGetLastError()
+    torch.cuda.synchronize()
+    assert kept and left == [0, 101] * 6, (kept, left)
+    assert (a.local_rows()[:5] == 4).all() and (a.local_rows()[5:2000] == 2).all()
+    assert (val[5] == 2).all() and (val[2000][:5] == 4).all() and (val[2000][5:] == 2).all()
+    assert (c.local_rows()[:2000] == 127).all()
+    world.wait_all()
