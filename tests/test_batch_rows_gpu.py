@@ -811,3 +811,68 @@ def test_earlier_errors_are_left(lam, world):
     assert (val[5] == 2).all() and (val[2000][:5] == 4).all() and (val[2000][5:] == 2).all()
     assert (c.local_rows()[:2000] == 127).all()
     world.wait_all()
+
+
+def check_training_steps(got, steps, start, w, scale, rate, drop=None):
+    """Whether the f32 rows `got` are within f32 arithmetic of the steps (indices, targets) in 64 bits; `drop`: a
+    record that the plain form leaves out of every step. The bound, with U half an f32 step, follows the steps:
+    a lookup is exact (scale is a power of two); a product of K terms, any order, is off by K U sum |x w|, the
+    subtraction and the division by one U of their results each, a value d w by the error of d and one U; a row's
+    sum, its scaling and the addition to the row as in ref.add; and the table's error so far goes through the
+    lookup."""
+    U = ref.U32 * (1 + 2.0 ** -10)
+    s, (n, k) = abs(ref.f32_of(-rate * scale)), (len(steps[0][0]), len(w))
+    exact, err, w = start.double(), torch.zeros(start.shape, dtype=torch.float64), w.double()
+    for i, y in steps:
+        y = y.double()
+        x = exact[i] * scale
+        z = x @ w - y
+        d = z / n
+        off = scale * err[i] @ w.abs() + U * (k * (x.abs() @ w.abs()) + z.abs())
+        off = off / n + U * d.abs()
+        v, voff = d[:, None] * w, off[:, None] * w.abs() + U * (d[:, None] * w).abs()
+        if drop is not None:
+            v[drop] = 0.0
+        total, size, far = (torch.zeros_like(exact).index_add_(0, i, t) for t in (v, v.abs(), voff))
+        count = torch.bincount(i, minlength=len(exact)).double()[:, None]
+        new = exact - s * total
+        err = err + s * far + U * (s * size * (count + 1) + (new.abs() + exact.abs()) * (count > 0))
+        exact = new
+    return bool(((got.cpu().double() - exact).abs() <= err).all())
+
+
+def test_training_steps_to_the_last_record(lam, world):
+    """Steps of a model that is a table and a vector, within the steps' own f32 bound: close enough to tell a
+    single missing record."""
+    g = gen(12)
+    rows, width, n, rate, scale = 300, 64, 800, 0.05, 0.5
+    t, w = torch.randn(rows, width, generator=g), torch.randn(width, generator=g)
+    table, steps = lam.RowArray.from_tensor(world.team(), t.cuda()), []
+    for _ in range(5):
+        i, y = indices(g, n, rows, "skewed"), torch.randn(n, generator=g)
+        x = table.batch_load_rows(i.cuda(), scale=scale).spawn().value()
+        d = (x @ w.cuda() - y.cuda()) / n
+        table.batch_add_rows(i.cuda(), d[:, None] * w.cuda(), scale=-rate * scale).block()
+        steps.append((i, y))
+    assert check_training_steps(table.local_rows(), steps, t, w, scale, rate)
+    for drop in (0, 17, n - 1):
+        assert not check_training_steps(table.local_rows(), steps, t, w, scale, rate, drop)
+
+
+@pytest.mark.parametrize("kind", FLOATS)
+@pytest.mark.parametrize("vals", FLOATS)
+@pytest.mark.parametrize("n,rows,width,how", [(1025, 300, 33, "any"), (2050, 4000, 520, "skewed"), (5000, 6000, 7, "distinct"),
+                                              (3000, 40, 1032, "few")])
+def test_store_floats_by_claims(lam, world, kind, vals, n, rows, width, how):
+    """More records than the scan of the list takes, of repeated rows, pads among them."""
+    g = gen(n)
+    a, t = float_array(lam, world, g, rows, width, kind)
+    for _ in range(2):                                   # the second call finds the claims that the first one left
+        i = indices(g, n, rows, how)
+        i[::7] = -1
+        v = torch.randn(n, width, generator=g).to(ref.TORCH[vals])
+        a.batch_store_rows(i.cuda(), v.cuda(), pad=-1).block()
+        last = ref.last_records(i, rows, -1)
+        at, rec = torch.tensor(list(last)), torch.tensor([last[r] for r in last])
+        t[at] = v[rec].to(ref.TORCH[kind])
+        assert torch.equal(a.local_rows().cpu(), t)
