@@ -370,7 +370,7 @@ class RowArray:
                 stride = rows.stride(0)
         stream = self._on_stream(k)
         if not alone:
-            self._exchange_load(k, idx, scale, rt, pad, rows, n)
+            self._exchange_load(k, idx, scale, rt, pad, rows, n, stride)
         elif n:
             k.rows_load(self._table, idx, n, pad, scale, rows, rt.code, stride, stream)
         if not fresh:
@@ -442,21 +442,21 @@ class RowArray:
         loc = loc.view(torch.int64)[:m].view(-1, 1) if m else gidx[:0].view(0, 1)
         return _all_to_all(self.team, loc, sent, got).view(-1), (pos if kept is None else kept[pos]), sent, got
 
-    def _exchange_load(self, k, idx, scale, rt, pad, rows, n):
+    def _exchange_load(self, k, idx, scale, rt, pad, rows, n, stride):
         mine, pos, sent, got = self._pack(k, idx, pad)
         reply = torch.empty(mine.numel(), self.row_len, dtype=rt.torch, device=k.device)
         if mine.numel():
             k.rows_load(self._table, mine, mine.numel(), None, scale, reply, rt.code, self.row_len, k.stream_id())
         reply = _all_to_all(self.team, reply, got, sent)
-        if pos.numel() < n:
-            rows.zero_()                                # pads, and what was out of bounds
-        if not pos.numel():
+        if n == 0:
             return
-        if rows.stride(0) == self.row_len or n == 1:
-            whole = _Table(rows, None, None, n, self.row_len, rt, None)
-            k.rows_store(whole, pos, pos.numel(), None, reply, rt.code, self.row_len, k.stream_id())
-        else:
-            rows[pos] = reply
+        # a lookup in what came back, whose order the pack decided: -1 for pads and what was out of bounds
+        m = pos.numel()
+        where = torch.full((n,), -1, dtype=torch.int64, device=k.device)
+        if m:
+            k.scatter_results(torch.arange(m, device=k.device), pos.to(torch.int32), m, 8, where)
+        back = _Table(reply, None, None, m, self.row_len, rt, None)
+        k.rows_load(back, where, n, -1, 1.0, rows, rt.code, stride, k.stream_id())
 
     def _exchange_values(self, k, idx, vals, pad):
         mine, pos, sent, got = self._pack(k, idx, pad)

@@ -328,6 +328,36 @@ def test_refused_numbers(lam, team):
     assert (a.local_rows()[3] == 5.5).all() and int((a.local_rows() != 0).sum()) == 6
 
 
+def test_exchange_places_rows_by_the_row_kernels(lam, monkeypatch):
+    """What comes back from the owners is put into `out`, whole or strided, pads and indices out of bounds as
+    zeros, by the row operators."""
+    from lamellar_runtime_amd import rows as rows_module
+    calls = []
+
+    class Kernels(CpuRowKernels):
+        def rows_load(self, table, idx, n, pad, scale, out, out_type, stride, stream):
+            calls.append((n, stride, out.data_ptr()))
+            super().rows_load(table, idx, n, pad, scale, out, out_type, stride, stream)
+
+    monkeypatch.setattr(rows_module, "_all_gather", lambda team, mine: [mine])
+    monkeypatch.setattr(rows_module, "_all_to_all", lambda team, rows, sent, got: rows)
+    team = lam.LamellarWorldBuilder().with_kernels(Kernels).build().team()
+    a = lam.RowArray.from_tensor(team, torch.arange(24.0).view(6, 4))
+    a._distributed = True
+    i = torch.tensor([5, -1, 0, 9, 5])
+    exp = torch.where(((i >= 0) & (i < 6))[:, None], a.local_rows()[i.clamp(0, 5)], 0.0)
+    wide = torch.full((5, 9), 7.0)
+    for out, stride in ((wide[:, 2:6], 9), (torch.full((5, 4), 7.0), 4)):
+        calls.clear()
+        h = a.batch_load_rows(i, pad=-1, out=out)
+        refused(lam, OOB, h.block)
+        assert torch.equal(h.value(), exp) and calls[-1] == (5, stride, out.data_ptr())
+    assert (wide[:, :2] == 7).all() and (wide[:, 6:] == 7).all()
+    got = a.batch_load_rows([[1], [4]], scale=2).block()
+    assert torch.equal(got[:, 0], a.local_rows()[[1, 4]] * 2)
+    assert not a.batch_load_rows([-1, -1], pad=-1).block().any()
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)
