@@ -323,11 +323,20 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     auto step = [&](const char* what) {
         if (dbg) fprintf(stderr, "[lmr_peer pe%u %.3f s] %s\n", t->me, now_s() - t_start, what);
     };
-    auto fail = [&](lmr_status_t st) {
+    // a machine may refuse any of these calls (host registration, uncached or shared memory): the
+    // message says which one it was, and PE 0 takes its segment back
+    bool made = false;
+    const char* why = "no answer in time";
+    auto fail = [&](const char* call) {
+        fprintf(stderr, "lmr_transport_peer_create: PE %u: %s failed: %s\n", t->me, call, why);
         peer_teardown(t);
-        if (t->me == 0 && t->shm) shm_unlink(t->name);
+        if (made) shm_unlink(t->name);
         delete t;
-        return st;
+        return LMR_E_HIP;
+    };
+    auto ok = [&](hipError_t e) {
+        if (e != hipSuccess) why = hipGetErrorString(e);
+        return e == hipSuccess;
     };
     step("mailbox");
     // ---- the mailbox: PE 0 creates the segment, the others open it
@@ -336,17 +345,22 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     if (t->me == 0) {
         shm_unlink(t->name);                                // a stale segment of a killed job
         fd = shm_open(t->name, O_CREAT | O_EXCL | O_RDWR, 0600);
+        made = fd >= 0;
         if (fd < 0 || ftruncate(fd, off_t(t->shm_bytes)) != 0) {
+            why = strerror(errno);
             if (fd >= 0) close(fd);
-            return fail(LMR_E_HIP);
+            return fail("shm_open of the mailbox");
         }
     } else if (!host_wait([&] { return (fd = shm_open(t->name, O_RDWR, 0600)) >= 0; }, to)) {
-        return fail(LMR_E_HIP);
+        return fail("the wait for the mailbox");
     }
     step("opened shm");
     void* m = mmap(nullptr, t->shm_bytes, PROT_READ | PROT_WRITE, MAP_SHARED, fd, 0);
     close(fd);
-    if (m == MAP_FAILED) return fail(LMR_E_HIP);
+    if (m == MAP_FAILED) {
+        why = strerror(errno);
+        return fail("mmap of the mailbox");
+    }
     t->shm = m;
     t->mb = carve(m, t->npes);
     if (t->me == 0) {
@@ -357,17 +371,17 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     } else {
         if (!host_wait([&] { return ld_acq(&t->mb.hdr->created) == 1 && t->mb.hdr->magic == kPeerMagic; }, to) ||
             t->mb.hdr->npes != t->npes)
-            return fail(LMR_E_HIP);
+            return fail("the wait for a mailbox of as many PEs");
     }
     step("mailbox ready");
     // device view of the mailbox (fine-grained: system-scope loads / stores cross GPUs and processes)
-    if (hipHostRegister(m, t->shm_bytes, hipHostRegisterMapped) != hipSuccess) {
+    if (!ok(hipHostRegister(m, t->shm_bytes, hipHostRegisterMapped))) {
         t->shm = nullptr;
         munmap(m, t->shm_bytes);
-        return fail(LMR_E_HIP);
+        return fail("hipHostRegister of the mailbox");
     }
     void* md = nullptr;
-    if (hipHostGetDevicePointer(&md, m, 0) != hipSuccess) return fail(LMR_E_HIP);
+    if (!ok(hipHostGetDevicePointer(&md, m, 0))) return fail("hipHostGetDevicePointer");
     t->mbd = carve(md, t->npes);
     step("registered");
     // ---- receive regions: [source][parity][index | values], R x 8 bytes each
@@ -382,24 +396,25 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     const unsigned mflags = (mk && mk[0] == 'f') ? hipDeviceMallocFinegrained : hipDeviceMallocUncached;
     t->local.assign(size_t(t->npes) * kRegionAllocs, nullptr);
     for (auto& l : t->local)
-        if (hipExtMallocWithFlags(reinterpret_cast<void**>(&l), t->R * 8, mflags) != hipSuccess) return fail(LMR_E_HIP);
+        if (!ok(hipExtMallocWithFlags(reinterpret_cast<void**>(&l), t->R * 8, mflags))) return fail("hipExtMallocWithFlags");
     step("regions allocated");
     PeSlot* mine = &t->mb.slots[t->me];
     for (uint32_t src = 0; src < t->npes; src++)
         for (int k = 0; k < kRegionAllocs; k++)
-            if (hipIpcGetMemHandle(&mine->handle[src][k], t->local[size_t(src) * kRegionAllocs + k]) != hipSuccess)
-                return fail(LMR_E_HIP);
+            if (!ok(hipIpcGetMemHandle(&mine->handle[src][k], t->local[size_t(src) * kRegionAllocs + k])))
+                return fail("hipIpcGetMemHandle");
     mine->region_recs = t->R;
     st_rel(&mine->ready, 1);
     step("handles exported");
     for (uint32_t p = 0; p < t->npes; p++) {
         PeSlot* s = &t->mb.slots[p];
-        if (!host_wait([&] { return ld_acq(&s->ready) == 1; }, to) || s->region_recs != t->R) return fail(LMR_E_HIP);
+        if (!host_wait([&] { return ld_acq(&s->ready) == 1; }, to) || s->region_recs != t->R)
+            return fail("the wait for every PE's regions of this size");
     }
     // the PEs map their regions at each other one PE at a time, in PE order, each through its first
     // kernel on the tables (8 processes sharing one GPU that imported at once stalled there)
     for (uint32_t p = 0; p < t->me; p++)
-        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].mapped) == 1; }, to)) return fail(LMR_E_HIP);
+        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].mapped) == 1; }, to)) return fail("the wait for this PE's turn");
     t->mapped.assign(size_t(t->npes) * kRegionAllocs, nullptr);
     for (uint32_t q = 0; q < t->npes; q++)
         for (int k = 0; k < kRegionAllocs; k++) {
@@ -409,8 +424,8 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
                 continue;
             }
             void* pp = nullptr;
-            if (hipIpcOpenMemHandle(&pp, t->mb.slots[q].handle[t->me][k], hipIpcMemLazyEnablePeerAccess) != hipSuccess)
-                return fail(LMR_E_HIP);
+            if (!ok(hipIpcOpenMemHandle(&pp, t->mb.slots[q].handle[t->me][k], hipIpcMemLazyEnablePeerAccess)))
+                return fail("hipIpcOpenMemHandle");
             dst = static_cast<uint8_t*>(pp);
         }
     step("peers mapped");
@@ -421,18 +436,18 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
             tab[size_t(b) * 2 * t->npes + q] = t->mapped[size_t(q) * kRegionAllocs + size_t(b) * 2];
             tab[(size_t(b) * 2 + 1) * t->npes + q] = t->mapped[size_t(q) * kRegionAllocs + size_t(b) * 2 + 1];
         }
-    if (hipMalloc(&t->d_tab, tab.size() * sizeof(uint8_t*)) != hipSuccess) return fail(LMR_E_HIP);
+    if (!ok(hipMalloc(&t->d_tab, tab.size() * sizeof(uint8_t*)))) return fail("hipMalloc");
     step("table allocated");
     PeerTabArgs ta{};
     for (size_t i = 0; i < tab.size(); i++) ta.p[i] = tab[i];
     hipLaunchKernelGGL(k_peer_tables, dim3(1), dim3(4 * kPeerMaxPes), 0, nullptr, ta, t->d_tab, uint32_t(tab.size()));
-    if (hipGetLastError() != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) return fail(LMR_E_HIP);
+    if (!ok(hipGetLastError()) || !ok(hipStreamSynchronize(nullptr))) return fail("k_peer_tables");
     step("tables");
     // the next PE maps only once this one's first kernel after its imports has completed
     st_rel(&mine->mapped, 1);
     st_rel(&mine->opened, 1);
     for (uint32_t p = 0; p < t->npes; p++)
-        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].opened) == 1; }, to)) return fail(LMR_E_HIP);
+        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].opened) == 1; }, to)) return fail("the wait for every PE");
     step("all opened");
     t->tp.num_pes = t->npes;
     t->tp.my_pe = t->me;

@@ -191,3 +191,24 @@ def test_staged_exchange_many_chunks(orc, ws, backend):
         exp2[fi] += pe[r]["gv"][:fi.size]
     for r in range(ws):
         assert np.array_equal(pe[r]["after_fetch"], exp2)
+
+
+def test_peer_transport_refused_names_the_call(capfd):
+    """A peer transport that cannot be made says which call failed and leaves no mailbox behind; where it can be
+    made, it is made and destroyed, and leaves none either."""
+    import ctypes
+    import glob
+
+    from _lamellar_bootstrap import load_package
+    load_package()
+    from lamellar_runtime_amd import _capi
+    job = f"t{os.getpid()}"
+    base = _capi.lmr_transport_t(num_pes=1, my_pe=0, host_buffers=1)
+    tp = ctypes.c_void_p()
+    st = _capi.lib().lmr_transport_peer_create(ctypes.byref(base), job.encode(), 4096, 0, ctypes.byref(tp))
+    said = capfd.readouterr().err
+    if st == 0:
+        assert _capi.lib().lmr_transport_peer_destroy(tp) == 0
+    else:
+        assert not tp.value and "lmr_transport_peer_create: PE 0: " in said and "hip" in said, said
+    assert not glob.glob(f"/dev/shm/lmr_peer_{job}*")
