@@ -132,13 +132,16 @@ class _Table:
         self.ptr = ctypes.addressof(self.c)
         self.lo = data.data_ptr()
         self.hi = self.lo + data.numel() * data.element_size()
+        self.scales_lo = scales.data_ptr() if scales is not None else 0
+        self.scales_hi = self.scales_lo + scales.numel() * 4 if scales is not None else 0
 
     def overlaps(self, t, n):
-        """Whether t (n rows of row_len) reaches into the table's rows."""
+        """Whether t (n rows of row_len) reaches into the table's rows or scales."""
         if n == 0:
             return False
         lo = t.data_ptr()
-        return lo < self.hi and self.lo < lo + ((n - 1) * t.stride(0) + self.row_len) * t.element_size()
+        hi = lo + ((n - 1) * t.stride(0) + self.row_len) * t.element_size()
+        return lo < self.hi and self.lo < hi or lo < self.scales_hi and self.scales_lo < hi
 
 
 class RowArray:

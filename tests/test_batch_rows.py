@@ -358,6 +358,26 @@ def test_exchange_places_rows_by_the_row_kernels(lam, monkeypatch):
     assert not a.batch_load_rows([-1, -1], pad=-1).block().any()
 
 
+def test_refused_memory(lam, team):
+    """Values and outputs that lie in the array's scales, as in its rows, are turned down: the batch would read
+    what it writes. Neighbours of either in one allocation are taken."""
+    mem = torch.zeros(100)
+    scales = mem[10:50].view(10, 4)
+    a = lam.RowArray.from_tensor(team, torch.zeros(10, 4, dtype=torch.int8), scales=scales)
+    for part in (scales, scales[2:5], mem[7:19].view(3, 4), mem[49:61].view(3, 4), mem[46:66].view(4, 5)[:, 1:], a.local_scales()[9:]):
+        i = list(range(len(part)))
+        refused(lam, INVALID, a.batch_store_rows(i, part).spawn)
+        refused(lam, INVALID, a.batch_load_rows(i, out=part).spawn)
+    refused(lam, INVALID, a.batch_store_rows([1, 2], scales[3]).spawn)
+    for part in (mem[2:10].view(2, 4), mem[50:58].view(2, 4)):
+        a.batch_store_rows([1, 2], part).block()
+        a.batch_load_rows([1, 2], out=part).block()
+    b = lam.RowArray.from_tensor(team, mem[60:80].view(5, 4))
+    refused(lam, INVALID, b.batch_add_rows([0], mem[76:80]).spawn)
+    refused(lam, INVALID, b.batch_load_rows([0], out=mem[57:61].view(1, 4)).spawn)
+    b.batch_add_rows([0], mem[80:84]).block()
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)
