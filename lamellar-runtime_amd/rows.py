@@ -168,7 +168,7 @@ class RowArray:
         on the team's device), shared, not copied. 8-bit codes come as int8, float8_e4m3fn, or uint8
         with `dtype`, and with `scales` (rows x groups, f32). `rows`: the rows of all PEs (the default:
         this PE's, at one PE)."""
-        if not isinstance(data, torch.Tensor) or data.dim() != 2 or not data.is_contiguous():
+        if not isinstance(data, torch.Tensor) or data.dim() != 2 or not data.is_contiguous() or data.is_neg():
             raise LamellarError(LmrStatus.INVALID, "from_tensor takes a contiguous 2-D tensor of rows")
         rt = row_type_of(data.dtype if dtype is None else dtype)
         if data.dtype != rt.torch and not (rt.is_code and data.dtype == torch.uint8):
@@ -336,6 +336,8 @@ class RowArray:
         if not isinstance(vals, torch.Tensor):
             vals = torch.from_numpy(np.ascontiguousarray(np.asarray(vals), dtype=np.float32))
         rt = _value_type(vals.dtype)
+        if vals.is_neg():
+            vals = vals.resolve_neg()
         if vals.shape == (n, self.row_len) and vals.device == k.device and vals.stride(1) == 1 and \
                 vals.stride(0) >= self.row_len:
             if self._table.overlaps(vals, n):
@@ -391,8 +393,9 @@ class RowArray:
             rows = out.detach().view(n, self.row_len)
         except RuntimeError:
             rows = None
-        if rows is None or (self.row_len > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < self.row_len):
-            raise LamellarError(LmrStatus.INVALID, f"out's rows are not contiguous and evenly spaced: strides {out.stride()}")
+        if rows is None or rows.is_neg() or (self.row_len > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < self.row_len):
+            raise LamellarError(LmrStatus.INVALID, "out's rows are not contiguous, evenly spaced and plain: strides "
+                                                   f"{out.stride()}{', negated' if out.is_neg() else ''}")
         if self._table.overlaps(rows, n):
             raise LamellarError(LmrStatus.INVALID, "out lies in the array's own memory")
         return rows

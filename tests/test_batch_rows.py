@@ -378,6 +378,37 @@ def test_refused_memory(lam, team):
     b.batch_add_rows([0], mem[80:84]).block()
 
 
+def test_negated_views(lam):
+    """Values that are a view whose sign torch keeps beside the memory (the imaginary part of a conjugate) are
+    taken with their sign; such an output is turned down."""
+
+    def raw(t):                                          # what the memory holds, as the device sees it
+        return torch._neg_view(t) if t.is_neg() else t
+
+    class Kernels(CpuRowKernels):
+        def rows_add(self, table, idx, n, pad, scale, vals, *a):
+            super().rows_add(table, idx, n, pad, scale, raw(vals), *a)
+
+        def rows_store(self, table, idx, n, pad, vals, *a):
+            super().rows_store(table, idx, n, pad, raw(vals), *a)
+
+    team = lam.LamellarWorldBuilder().with_kernels(Kernels).build().team()
+    for width in (1, 4):
+        a = lam.RowArray(team, 5, width)
+        v = torch.complex(torch.zeros(3, width), torch.ones(3, width)).conj().imag
+        assert v.is_neg() and (v == -1).all()
+        for vals in (v, torch._neg_view(torch.ones(3, width)), v[:1]):
+            a.local_rows().zero_()
+            i = list(range(len(vals)))
+            a.batch_add_rows(i, vals, scale=2).block()
+            assert (a.local_rows()[i] == -2).all()
+            a.batch_store_rows(i, vals).block()
+            assert (a.local_rows()[i] == -1).all()
+        for out in (torch._neg_view(torch.ones(3, width)),):
+            refused(lam, INVALID, a.batch_load_rows([0, 1, 2], out=out).spawn)
+    refused(lam, INVALID, lam.RowArray.from_tensor, team, torch._neg_view(torch.ones(3, 4)))
+
+
 # ------------------------------------------------------------------ several PEs
 def _inputs(rank, n, rows, width, seed):
     g = torch.Generator().manual_seed(seed * 10 + rank)
