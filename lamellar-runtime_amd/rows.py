@@ -444,7 +444,7 @@ class RowArray:
                                                        f"{MAX_BATCH}, of {MAX_VALUES} elements)")
         got = [e[1 + self.team.my_pe()] for e in every]
         m = sum(sent)                                   # an index out of bounds is dropped there
-        pos = pos[:m].to(torch.int64)
+        pos = pos[:m]
         loc = loc.view(torch.int64)[:m].view(-1, 1) if m else gidx[:0].view(0, 1)
         return _all_to_all(self.team, loc, sent, got).view(-1), (pos if kept is None else kept[pos]), sent, got
 
@@ -456,11 +456,18 @@ class RowArray:
         reply = _all_to_all(self.team, reply, got, sent)
         if n == 0:
             return
-        # a lookup in what came back, whose order the pack decided: -1 for pads and what was out of bounds
         m = pos.numel()
-        where = torch.full((n,), -1, dtype=torch.int64, device=k.device)
+        if stride == self.row_len:
+            if m < n:
+                rows.zero_()                            # pads, and what was out of bounds
+            whole = _Table(rows, None, None, n, self.row_len, rt, None)
+            if m:
+                k.rows_store(whole, pos, m, None, reply, rt.code, self.row_len, k.stream_id())
+            return
+        # strided rows: a lookup in what came back, -1 for those that get zeros
+        where = torch.empty(n, dtype=torch.int64, device=k.device) if m == n else torch.full((n,), -1, dtype=torch.int64, device=k.device)
         if m:
-            k.scatter_results(torch.arange(m, device=k.device), pos.to(torch.int32), m, 8, where)
+            k.scatter_results(torch.arange(m, device=k.device), pos if pos.dtype == torch.int32 else pos.to(torch.int32), m, 8, where)
         back = _Table(reply, None, None, m, self.row_len, rt, None)
         k.rows_load(back, where, n, -1, 1.0, rows, rt.code, stride, k.stream_id())
 

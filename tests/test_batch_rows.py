@@ -336,8 +336,12 @@ def test_exchange_places_rows_by_the_row_kernels(lam, monkeypatch):
 
     class Kernels(CpuRowKernels):
         def rows_load(self, table, idx, n, pad, scale, out, out_type, stride, stream):
-            calls.append((n, stride, out.data_ptr()))
+            calls.append(out.data_ptr())
             super().rows_load(table, idx, n, pad, scale, out, out_type, stride, stream)
+
+        def rows_store(self, table, *a):
+            calls.append(table.data.data_ptr())
+            super().rows_store(table, *a)
 
     monkeypatch.setattr(rows_module, "_all_gather", lambda team, mine: [mine])
     monkeypatch.setattr(rows_module, "_all_to_all", lambda team, rows, sent, got: rows)
@@ -347,11 +351,11 @@ def test_exchange_places_rows_by_the_row_kernels(lam, monkeypatch):
     i = torch.tensor([5, -1, 0, 9, 5])
     exp = torch.where(((i >= 0) & (i < 6))[:, None], a.local_rows()[i.clamp(0, 5)], 0.0)
     wide = torch.full((5, 9), 7.0)
-    for out, stride in ((wide[:, 2:6], 9), (torch.full((5, 4), 7.0), 4)):
+    for out in (wide[:, 2:6], torch.full((5, 4), 7.0)):
         calls.clear()
         h = a.batch_load_rows(i, pad=-1, out=out)
         refused(lam, OOB, h.block)
-        assert torch.equal(h.value(), exp) and calls[-1] == (5, stride, out.data_ptr())
+        assert torch.equal(h.value(), exp) and calls[-1] == out.data_ptr()
     assert (wide[:, :2] == 7).all() and (wide[:, 6:] == 7).all()
     got = a.batch_load_rows([[1], [4]], scale=2).block()
     assert torch.equal(got[:, 0], a.local_rows()[[1, 4]] * 2)
