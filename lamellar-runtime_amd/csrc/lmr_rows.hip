@@ -47,7 +47,8 @@ __device__ __forceinline__ int64_t row_of(const RowBatch& b, uint64_t t, uint64_
 // the row's chunks (one in 64 bits per block, one in 32 per chunk, both multiplications). The result is
 // written past the caches' reuse order: it is as large as the table's rows or larger, and read once
 // (65536 bf16 rows of 4096: 142 us against 159 through the caches, and 158, 144, 142, 146 us with U = 1,
-// 2, 4, 8). Now 133 us, 5.3 TB/s; 262144 e4m3 rows of 1024 to bf16 141 us, 5.8 TB/s; 16 rows 2.6 us.
+// 2, 4, 8). Now 134 us, 5.3 TB/s (medians here and below); 262144 e4m3 rows of 1024 to bf16 142 us, 5.7 TB/s;
+// 16 rows 2.6 us. Groups that are no multiple of 8 (65536 e4m3 rows of 1000, groups of 100) 37 us, 5.4 TB/s.
 // GA: groups of a multiple of 8 elements, so that a chunk has one scale.
 template <typename T, typename O, int IW, int U, bool GA>
 __global__ __launch_bounds__(256) void k_rows_load(RowTable tab, RowBatch b, O* out, uint32_t* err, Divisor cpr, Divisor cpg) {
@@ -497,7 +498,7 @@ __global__ __launch_bounds__(1024) void k_rows_merge(SortPass p, uint32_t part) 
 // whose records begin in the tile and end there or in the next one is summed by this group alone and
 // added to the table at once. Only longer runs are cut: their parts go to `last` (the tile in which
 // they begin) and `first` (every later one), and k_rows_join adds them up. Every value is read once and
-// every named row read and written once: 131072 bf16 records of 4096 into f32 take 443 us here (4.9 TB/s
+// every named row read and written once: 131072 bf16 records of 4096 into f32 take 446 us here (4.9 TB/s
 // of the 2.2 GB that must move) of 496 in all.
 struct SumArgs {
     const uint2* rec;     // sorted (row, record)
@@ -601,7 +602,9 @@ __global__ __launch_bounds__(256) void k_rows_sum(RowTable tab, RowBatch b, cons
 // that `lanes` lanes hold, its lane groups a share of the parts each. Where there are many parts (one row
 // may have every record) the block does it together. Few lanes, so that the parts of one row are read by
 // as many compute units as its columns allow (8192 records of 512 columns, all of one row: 64, 45, 35 us
-// with 64, 32, 16 lanes; 131072 of 4096 as tokens come: 502, 502, 506). The list's order is no one's:
+// with 64, 32, 16 lanes; 131072 of 4096 as tokens come: 502, 502, 506). A long run of few columns is left to
+// few of them all the same: 131072 records of 64 columns, all of one row, take 80 us in all, 42 of even rows;
+// 2^20 of 128 255 and 138. The list's order is no one's:
 // every row is in it once, and its parts are added in an order that their number fixes.
 constexpr uint32_t kWaveParts = 64;
 constexpr uint32_t kJoinWaves = 8;
@@ -743,7 +746,9 @@ __device__ __forceinline__ Chunk<T> pack_codes(const float (&v)[kChunk], const G
 // L lanes per record: 8 to 64 (as many as hold a short row, so that a wave takes several), or the whole
 // block. Groups of up to 512 elements: as many lanes as hold one (a power of two) find its largest |x|
 // by shuffles and keep its values in registers. Longer groups are read twice, the second time from cache.
-// 16384 bf16 rows of 2048 to i8: 22 us, 4.6 TB/s; 65536 rows of 64 to e4m3 10 us (26 with a wave for each).
+// 16384 bf16 rows of 2048 to i8: 24 us, 4.2 TB/s; 65536 rows of 64 to e4m3 10 us (26 with a wave for each). With
+// the claims' launch, 65536 bf16 rows: of 1024 in groups of 128 to e4m3 41 us, 5.0 TB/s; of 1000 in groups of 100
+// 48 us, 4.1; of 1152 in groups of 576 62 us, 3.7 (to i8 67, 3.4); of 4096 to bf16 217 us, 5.0 TB/s, of 64 11 us.
 template <typename T, typename V, int IW, int L>
 __global__ __launch_bounds__(256) void k_rows_store(RowTable tab, RowBatch b, const V* vals, uint32_t* err, int how, uint32_t lpg) {
     constexpr int kWaves = L > 64 ? L / 64 : 1;                    // waves that share a record

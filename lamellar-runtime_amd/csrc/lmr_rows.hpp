@@ -136,8 +136,8 @@ __device__ __forceinline__ Chunk<T> pack(const float (&v)[kChunk]) {
     return c;
 }
 
-// x / d for x < 2^45 (64 bits) and x < 2^17 (32 bits), d < 2^16: multiplication by 2^64 / d (2^32 / d)
-// rounded up is exact while x * d stays below 2^64 (2^32)
+// x / d by multiplication with 2^64 / d (2^32 / d) rounded up: exact while x * d stays below 2^64 (2^32).
+// Here d is at most 2^15 (the chunks of the longest row) and x below 2^34, 2^16 where it has 32 bits.
 struct Divisor { uint32_t d, m32; uint64_t m64; };
 inline Divisor divisor(uint32_t d) {
     return {d, d > 1 ? uint32_t((uint64_t(1) << 32) / d + 1) : 0u, d > 1 ? ~uint64_t(0) / d + 1 : 0u};
