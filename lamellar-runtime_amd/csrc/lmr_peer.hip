@@ -50,14 +50,16 @@ struct PeSlot {
     int64_t info[2][kInfoWords];
     uint64_t closing;
     uint64_t mapped;                      // 1: this PE's hipIpcOpenMemHandle calls are done
-    uint64_t pad[4];
+    uint64_t seen;                        // 1: this PE has mapped the mailbox
+    uint64_t pad[3];
 };
 
 struct MbHeader {
     uint64_t magic;
     uint64_t npes;
     uint64_t created;
-    uint64_t pad[5];
+    uint64_t refused;                     // 1: some PE's set-up failed: nobody waits for it any longer
+    uint64_t pad[4];
 };
 
 // mailbox flag arrays, index (owner q, source p, parity b) = (q * npes + p) * 2 + b
@@ -324,16 +326,31 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
         if (dbg) fprintf(stderr, "[lmr_peer pe%u %.3f s] %s\n", t->me, now_s() - t_start, what);
     };
     // a machine may refuse any of these calls (host registration, uncached or shared memory): the
-    // message says which one it was, and PE 0 takes its segment back
-    bool made = false;
-    const char* why = "no answer in time";
+    // message says which one it was, the mailbox tells the other PEs, and PE 0 takes the segment back
+    // once all of them have it (one that came later would wait for it)
+    bool made = false, registered = false;
+    const char* why = nullptr;                             // null: a wait
+    auto refused = [&] { return t->mb.hdr && ld_acq(&t->mb.hdr->refused) == 1; };
     auto fail = [&](const char* call) {
-        fprintf(stderr, "lmr_transport_peer_create: PE %u: %s failed: %s\n", t->me, call, why);
+        fprintf(stderr, "lmr_transport_peer_create: PE %u: %s failed: %s\n", t->me, call,
+                why ? why : refused() ? "another PE's set-up failed" : "no answer in time");
+        if (t->shm) {
+            st_rel(&t->mb.hdr->refused, 1);
+            for (uint32_t p = 0; made && p < t->npes; p++)
+                if (p != t->me) (void)host_wait([&] { return ld_acq(&t->mb.slots[p].seen) == 1; }, to);
+            if (!registered) {
+                munmap(t->shm, t->shm_bytes);
+                t->shm = nullptr;
+            }
+        }
+        t->mb = Mailbox{};
         peer_teardown(t);
         if (made) shm_unlink(t->name);
         delete t;
         return LMR_E_HIP;
     };
+    // until pred() holds: false when time runs out or a PE's set-up has failed
+    auto wait_for = [&](auto pred) { return host_wait([&] { return pred() || refused(); }, to) && pred(); };
     auto ok = [&](hipError_t e) {
         if (e != hipSuccess) why = hipGetErrorString(e);
         return e == hipSuccess;
@@ -373,13 +390,11 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
             t->mb.hdr->npes != t->npes)
             return fail("the wait for a mailbox of as many PEs");
     }
+    st_rel(&t->mb.slots[t->me].seen, 1);
     step("mailbox ready");
     // device view of the mailbox (fine-grained: system-scope loads / stores cross GPUs and processes)
-    if (!ok(hipHostRegister(m, t->shm_bytes, hipHostRegisterMapped))) {
-        t->shm = nullptr;
-        munmap(m, t->shm_bytes);
-        return fail("hipHostRegister of the mailbox");
-    }
+    if (!ok(hipHostRegister(m, t->shm_bytes, hipHostRegisterMapped))) return fail("hipHostRegister of the mailbox");
+    registered = true;
     void* md = nullptr;
     if (!ok(hipHostGetDevicePointer(&md, m, 0))) return fail("hipHostGetDevicePointer");
     t->mbd = carve(md, t->npes);
@@ -408,13 +423,13 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     step("handles exported");
     for (uint32_t p = 0; p < t->npes; p++) {
         PeSlot* s = &t->mb.slots[p];
-        if (!host_wait([&] { return ld_acq(&s->ready) == 1; }, to) || s->region_recs != t->R)
+        if (!wait_for([&] { return ld_acq(&s->ready) == 1; }) || s->region_recs != t->R)
             return fail("the wait for every PE's regions of this size");
     }
     // the PEs map their regions at each other one PE at a time, in PE order, each through its first
     // kernel on the tables (8 processes sharing one GPU that imported at once stalled there)
     for (uint32_t p = 0; p < t->me; p++)
-        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].mapped) == 1; }, to)) return fail("the wait for this PE's turn");
+        if (!wait_for([&] { return ld_acq(&t->mb.slots[p].mapped) == 1; })) return fail("the wait for this PE's turn");
     t->mapped.assign(size_t(t->npes) * kRegionAllocs, nullptr);
     for (uint32_t q = 0; q < t->npes; q++)
         for (int k = 0; k < kRegionAllocs; k++) {
@@ -447,7 +462,7 @@ lmr_status_t lmr_transport_peer_create(const lmr_transport_t* base, const char* 
     st_rel(&mine->mapped, 1);
     st_rel(&mine->opened, 1);
     for (uint32_t p = 0; p < t->npes; p++)
-        if (!host_wait([&] { return ld_acq(&t->mb.slots[p].opened) == 1; }, to)) return fail("the wait for every PE");
+        if (!wait_for([&] { return ld_acq(&t->mb.slots[p].opened) == 1; })) return fail("the wait for every PE");
     step("all opened");
     t->tp.num_pes = t->npes;
     t->tp.my_pe = t->me;

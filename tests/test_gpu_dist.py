@@ -212,3 +212,38 @@ def test_peer_transport_refused_names_the_call(capfd):
     else:
         assert not tp.value and "lmr_transport_peer_create: PE 0: " in said and "hip" in said, said
     assert not glob.glob(f"/dev/shm/lmr_peer_{job}*")
+
+
+REFUSED_WORKER = r'''
+import ctypes, os, sys, time
+sys.path.insert(0, os.environ["LMR_ROOT"])
+from _lamellar_bootstrap import load_package
+load_package()
+from lamellar_runtime_amd import _capi
+import torch
+torch.zeros(1, device="cuda")
+me = int(sys.argv[1])
+time.sleep(3 * me)                      # PE 0 is through with the call before the others begin
+base = _capi.lmr_transport_t(num_pes=2, my_pe=me, host_buffers=1)
+tp = ctypes.c_void_p()
+t0 = time.monotonic()
+st = _capi.lib().lmr_transport_peer_create(ctypes.byref(base), sys.argv[2].encode(), 4096, 0, ctypes.byref(tp))
+print("took", time.monotonic() - t0, "status", st, flush=True)
+if st == 0:
+    assert _capi.lib().lmr_transport_peer_destroy(tp) == 0
+'''
+
+
+def test_peer_transport_refused_by_one_refuses_all():
+    """Where one PE cannot make the transport, the others learn of it and do not wait for their time to run out;
+    the mailbox goes when all have seen it."""
+    import glob
+    job = f"u{os.getpid()}"
+    env = dict(os.environ, LMR_ROOT=ROOT, LAMELLAR_PEER_TIMEOUT="40")
+    procs = [subprocess.Popen([sys.executable, "-c", REFUSED_WORKER, str(r), job], env=env, stdout=subprocess.PIPE, text=True)
+             for r in range(2)]
+    out = [p.communicate(timeout=100)[0] for p in procs]
+    assert [p.returncode for p in procs] == [0, 0], out
+    took = [float(o.split("took ")[1].split()[0]) for o in out]
+    assert out[0].split("status ")[1] == out[1].split("status ")[1] and max(took) < 20, out
+    assert not glob.glob(f"/dev/shm/lmr_peer_{job}*")
